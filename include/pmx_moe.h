@@ -379,6 +379,87 @@ int pmx_decode_cache_attention(const void* query, const void* current_key, const
                                int64_t kv_stride, int64_t head_stride, int64_t max_kvlen,
                                int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Rotary positions on packed heads, optionally behind an RMS norm of every head.  Token t of
+ * sequence b (seqstarts[b] <= t < seqstarts[b+1]) is at position start_pos[b] + t - seqstarts[b], or at
+ * position_ids[t] where that is given.  Pair i of the first rotary_dim values, a = position * frequencies[i]:
+ *   (x1, x2) -> factor * (x1 cos a - x2 sin a, x2 cos a + x1 sin a)
+ * pairs (i, i + rotary_dim/2), or (2i, 2i+1) when interleaved; with norm weights [head_dim] x is first
+ * x * weight / sqrt(mean(x^2) + eps) over the head (all head_dim values).  Tokens of no sequence are copied.
+ * fp32 arithmetic (angles in 64 bits), one rounding.  query [T, num_heads, head_dim], key [T, num_kv_heads,
+ * head_dim] or NULL with num_kv_heads 0, both with the given strides in elements and unit inner stride;
+ * outputs dense.  frequencies: HOST array of rotary_dim/2 doubles.  rotary_dim even, at most 256.
+ * All three dtypes; any alignment and stride (16-byte aligned rows run the vector kernel).
+ */
+int pmx_rotary_embedding(const void* query, const void* key, const void* query_norm_weight,
+                         const void* key_norm_weight, float eps, void* query_out, void* key_out,
+                         const int64_t* seqstarts, const int64_t* start_pos, const int64_t* position_ids, int64_t T,
+                         int32_t B, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                         int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                         int64_t k_head_stride, const double* frequencies, int32_t rotary_dim, float factor,
+                         int32_t interleaved, int32_t dtype, void* stream);
+
+/*
+ * Attention of packed ragged prompts.  Sequence b has the queries seqstarts[b] .. seqstarts[b+1] and the keys
+ * kvstarts[b] .. kvstarts[b+1]; its queries are the LAST of its positions.  With is_causal a query at position i
+ * sees the keys j <= i and, with prefix_lens, those j < prefix_lens[b]; otherwise all of its sequence.
+ *   s = scale q.k;  logit_cap c > 0: s = c tanh(s / c);  alibi_slopes [num_heads]: s -= slope |i - j|;
+ *   out = softmax(s) v over the keys seen; a query that sees none, and a row of no sequence, is zero.
+ * What a query may not see does not reach its result, whatever it holds (infinities and NaN included).
+ * seqstarts, kvstarts [B+1], prefix_lens [B] int64 on the device; max_seqlen / max_kvlen: at least the longest
+ * sequence's queries / keys (host values that size the grid).  head_dim at most 256.  16-bit tensors with
+ * head_dim a multiple of 8 up to 128, 16-byte aligned rows and at most 128 query heads per kv head run on the
+ * tensor cores, other calls on a plain kernel.  fp32 softmax and sums; on the tensor cores the
+ * probabilities are rounded to the inputs' type for the second product.
+ */
+size_t pmx_prompt_attention_workspace_bytes(int64_t Tq, int32_t B, int32_t num_heads, int32_t num_kv_heads,
+                                            int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype);
+int pmx_prompt_attention(const void* query, const void* key, const void* value, const int64_t* seqstarts,
+                         const int64_t* kvstarts, const int64_t* prefix_lens, const float* alibi_slopes, void* out,
+                         int64_t Tq, int64_t Tk, int32_t B, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                         int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t v_token_stride, int64_t v_head_stride, int64_t max_seqlen, int64_t max_kvlen,
+                         int32_t is_causal, float scale, float logit_cap, int32_t dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of drafted tokens over the cache.  Sequence b brings seqstarts[b+1] - seqstarts[b] <= 64 drafted
+ * tokens; their keys and values are stored at cache rows cachestarts[b] + start_pos[b] + i, and token i sees the
+ * start_pos[b] cached rows and the drafted tokens j of its sequence with bit j of tree_mask[token] set (its own
+ * bit included, if it is to see itself).  Scores, empty rows, types and kernels as for pmx_prompt_attention;
+ * cache strides as for pmx_decode_cache_attention, cache_rows rows in all (new rows outside are not stored).
+ */
+size_t pmx_tree_cache_attention_workspace_bytes(int64_t Tq, int32_t B, int32_t num_heads, int32_t num_kv_heads,
+                                                int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype);
+int pmx_tree_cache_attention(const void* query, const void* current_key, const void* current_value, void* cache,
+                             const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
+                             const int64_t* tree_mask, void* out, int64_t Tq, int32_t B, int32_t num_heads,
+                             int32_t num_kv_heads, int32_t head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                             int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                             int64_t v_head_stride, int64_t cache_rows, int64_t layer_offset, int64_t row_stride,
+                             int64_t kv_stride, int64_t head_stride, int64_t max_seqlen, int64_t max_kvlen, float scale,
+                             float logit_cap, int32_t dtype, void* workspace, size_t workspace_bytes,
+                             void* stream);
+/* Synchronises `stream`; PMX_ERR_DEVICE_CHECK (out = code, role, tile, CTA) if a bounded wait inside one of the two
+ * attention kernels ran out on the current device since the last check (their results are then undefined), and
+ * clears the record. */
+int pmx_attention_check(int32_t out[4], void* stream);
+
+/*
+ * After verification: the accepted drafted rows move to the front of the drafted range.  For i <
+ * accept_starts[b+1] - accept_starts[b] (at most max_accept <= 64), in every layer, keys and values:
+ *   cache row base + i <- cache row base + accept_index[accept_starts[b] + i],  base = cachestarts[b] + start_pos[b],
+ * all rows of a sequence read before any is written, so the indices may come in any order and repeat.  A
+ * negative index, and a row outside the cache_rows rows, is skipped.  index_count: entries of accept_index.  The
+ * cache element (row, layer, kv, head, d) lies at row*row_stride + layer*layer_stride + kv*kv_stride +
+ * head*head_stride + d.
+ */
+int pmx_compact_cache(void* cache, const int64_t* cachestarts, const int64_t* start_pos, const int64_t* accept_starts,
+                      const int64_t* accept_index, int64_t B, int64_t index_count, int32_t max_accept,
+                      int32_t num_layers, int32_t num_kv_heads, int32_t head_dim, int64_t cache_rows,
+                      int64_t row_stride, int64_t layer_stride, int64_t kv_stride, int64_t head_stride, int32_t dtype,
+                      void* stream);
+
 /* how pmx_moe_reduce_allreduce moves the partial results between the ranks */
 typedef enum pmx_allreduce_algorithm {
   PMX_ALLREDUCE_AUTO = 0,

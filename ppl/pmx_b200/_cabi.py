@@ -80,6 +80,18 @@ def _load() -> C.CDLL:
         "pmx_decode_cache_attention_workspace_bytes": (sz, [i64, i32, i32, i32, i64]),
         "pmx_decode_cache_attention": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i64, i64, i64, i64, i64,
                                                  i32, vp, sz, vp]),
+        "pmx_rotary_embedding": (C.c_int, [vp, vp, vp, vp, f32, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i64, i64,
+                                           i64, i64, vp, i32, f32, i32, i32, vp]),
+        "pmx_prompt_attention_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64, i64, i32]),
+        "pmx_prompt_attention": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, i32, i64, i64, i64,
+                                           i64, i64, i64, i64, i64, i32, f32, f32, i32, vp, sz, vp]),
+        "pmx_tree_cache_attention_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64, i64, i32]),
+        "pmx_tree_cache_attention": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i64, i64,
+                                               i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, f32, f32, i32, vp,
+                                               sz, vp]),
+        "pmx_attention_check": (C.c_int, [C.POINTER(i32 * 4), vp]),
+        "pmx_compact_cache": (C.c_int, [vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, i32, i64, i64, i64, i64, i64, i32,
+                                        vp]),
         "pmx_moe_reduce_allreduce_buffer_bytes": (sz, [i64, i64, i32]),
         "pmx_moe_reduce_allreduce": (C.c_int, [vp, vp, vp, vp, i64, i32, i64, i32, C.POINTER(vp), i32, i32, sz,
                                                i32, i32, i64, vp]),

@@ -1,4 +1,6 @@
-"""`pmx_llm.torch_function.dynamic_batching` operators covered by this package.
+"""`pmx_llm.torch_function.dynamic_batching` operators covered by this package, and the operators
+that a decoder's attention block needs around them: rotary positions (rotary.py), attention of prompts
+and of drafted trees (masked_attention.py), moving accepted rows in the cache (cache_rows.py).
 
 `multi_head_cache_attention` keeps the signature, output layout and ONNX custom-op export of
 the reference operator (torch_function/dynamic_batching/MultiHeadCacheAttention.py:13-147) for
@@ -140,3 +142,14 @@ def multi_head_cache_attention(query: torch.Tensor, current_key: torch.Tensor, c
                                          start_pos, decoding_batches, max_seqlen, max_kvlen, cache, scale, attn_mask,
                                          num_heads, head_dim, is_causal, is_alibi, num_kv_heads, num_layer, layer_idx,
                                          quant_bit, quant_group, cache_mode, cache_layout, page_size)
+
+
+from .rotary import (rotary_position_embedding, qk_norm_rotary_embedding, rotary_frequencies, RotaryPositionEmbedding,  # noqa: E402
+                     QkNormRotaryEmbedding)
+from .masked_attention import (prompt_attention, tree_cache_attention, attention_check, PromptAttention,  # noqa: E402
+                               TreeCacheAttention)
+from .cache_rows import compact_cache  # noqa: E402
+
+__all__ = ["multi_head_cache_attention", "set_decode_attention_kernel", "cache_strides", "rotary_position_embedding",
+           "qk_norm_rotary_embedding", "rotary_frequencies", "prompt_attention", "tree_cache_attention",
+           "attention_check", "compact_cache"]
