@@ -194,6 +194,11 @@ int launch_rows(const AttnArgs& a, int dtype, const char* name, cudaStream_t s) 
   }
 }
 
+#include "tcgen05_common.cuh"
+namespace tc {
+#include "masked_attention_tc.cuh"
+}
+
 int check_common(const AttnArgs& a, int dtype, const char* name) {
   if (a.Tq <= 0 || a.B <= 0 || a.Hq <= 0 || a.Hkv <= 0 || a.D <= 0 || a.max_seqlen <= 0 || a.Hq % a.Hkv)
     return fail(PMX_ERR_INVALID_ARGUMENT, "%s: sizes must be positive and num_heads a multiple of num_kv_heads (tokens=%lld B=%d heads=%d/%d)", name, (long long)a.Tq, a.B, a.Hq, a.Hkv);
@@ -208,23 +213,26 @@ int check_common(const AttnArgs& a, int dtype, const char* name) {
 
 }  // namespace
 
-// record of a bounded wait that ran out: code, role, tile, CTA
-__device__ int g_attention_status[4];
-
 int attention_check(int out[4], cudaStream_t s) {
-  PMX_CUDA_OK(cudaMemcpyFromSymbolAsync(out, g_attention_status, sizeof(g_attention_status), 0, cudaMemcpyDeviceToHost, s));
+  PMX_CUDA_OK(cudaMemcpyFromSymbolAsync(out, tc::g_attention_status, sizeof(tc::g_attention_status), 0, cudaMemcpyDeviceToHost, s));
   PMX_CUDA_OK(cudaStreamSynchronize(s));
   if (out[0] == 0) return PMX_OK;
   void* at = nullptr;
-  PMX_CUDA_OK(cudaGetSymbolAddress(&at, g_attention_status));
-  PMX_CUDA_OK(cudaMemsetAsync(at, 0, sizeof(g_attention_status), s));
+  PMX_CUDA_OK(cudaGetSymbolAddress(&at, tc::g_attention_status));
+  PMX_CUDA_OK(cudaMemsetAsync(at, 0, sizeof(tc::g_attention_status), s));
   PMX_CUDA_OK(cudaStreamSynchronize(s));
   return fail(PMX_ERR_DEVICE_CHECK, "attention: a wait inside a kernel ran out (role %d, tile %d, CTA %d)", out[1], out[2], out[3]);
 }
 
-size_t prompt_attention_workspace_bytes(int64_t, int, int, int, int, int64_t, int64_t, int) { return 16; }
+size_t prompt_attention_workspace_bytes(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, int64_t max_kvlen,
+                                        int dtype) {
+  return tc::tc_workspace(tc::plan_tc(Tq, B, Hq, Hkv, D, max_seqlen, max_kvlen, dtype), Tq, Hq, D);
+}
 
-size_t tree_attention_workspace_bytes(int64_t, int, int, int, int, int64_t, int64_t, int) { return 16; }
+size_t tree_attention_workspace_bytes(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, int64_t max_kvlen,
+                                        int dtype) {
+  return tc::tc_workspace(tc::plan_tc(Tq, B, Hq, Hkv, D, max_seqlen, max_kvlen, dtype), Tq, Hq, D);
+}
 
 int launch_prompt_attention(const PromptAttention& p, void* ws, size_t ws_bytes, cudaStream_t s) {
   const char* name = "prompt_attention";
@@ -241,7 +249,9 @@ int launch_prompt_attention(const PromptAttention& p, void* ws, size_t ws_bytes,
   if (st != PMX_OK) return st;
   const size_t need = prompt_attention_workspace_bytes(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype);
   if (!ws || ws_bytes < need) return fail(PMX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", name, need, ws_bytes);
-  return launch_rows(a, p.dtype, name, s);
+  bool done;
+  const int tc_status = tc::launch_tc(a, tc::plan_tc(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype), p.dtype, name, ws, s, &done);
+  return done ? tc_status : launch_rows(a, p.dtype, name, s);
 }
 
 int launch_tree_attention(const TreeAttention& p, void* ws, size_t ws_bytes, cudaStream_t s) {
@@ -264,7 +274,9 @@ int launch_tree_attention(const TreeAttention& p, void* ws, size_t ws_bytes, cud
   if (st != PMX_OK) return st;
   const size_t need = tree_attention_workspace_bytes(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype);
   if (!ws || ws_bytes < need) return fail(PMX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", name, need, ws_bytes);
-  return launch_rows(a, p.dtype, name, s);
+  bool done;
+  const int tc_status = tc::launch_tc(a, tc::plan_tc(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype), p.dtype, name, ws, s, &done);
+  return done ? tc_status : launch_rows(a, p.dtype, name, s);
 }
 
 }  // namespace pmx
