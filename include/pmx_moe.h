@@ -391,13 +391,17 @@ int pmx_decode_cache_attention(const void* query, const void* current_key, const
  * outputs dense.  frequencies: HOST array of rotary_dim/2 doubles.  rotary_dim even, at most 256.
  * All three dtypes; any alignment and stride (16-byte aligned rows run the vector kernel).
  */
-int pmx_rotary_embedding(const void* query, const void* key, const void* query_norm_weight,
-                         const void* key_norm_weight, float eps, void* query_out, void* key_out,
-                         const int64_t* seqstarts, const int64_t* start_pos, const int64_t* position_ids, int64_t T,
-                         int32_t B, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                         int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
-                         int64_t k_head_stride, const double* frequencies, int32_t rotary_dim, float factor,
-                         int32_t interleaved, int32_t dtype, void* stream);
+typedef struct pmx_rotary_args {        /* every member 8 bytes wide, here and below */
+  const void *query, *key, *query_norm_weight, *key_norm_weight;
+  void *query_out, *key_out;
+  const int64_t *seqstarts, *start_pos, *position_ids;
+  const double* frequencies;
+  int64_t tokens, sequences, num_heads, num_kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t rotary_dim, interleaved, dtype;
+  double eps, factor;
+} pmx_rotary_args;
+int pmx_rotary_embedding(const pmx_rotary_args* args, void* stream);
 
 /*
  * Attention of packed ragged prompts.  Sequence b has the queries seqstarts[b] .. seqstarts[b+1] and the keys
@@ -412,15 +416,20 @@ int pmx_rotary_embedding(const void* query, const void* key, const void* query_n
  * tensor cores, other calls on a plain kernel.  fp32 softmax and sums; on the tensor cores the
  * probabilities are rounded to the inputs' type for the second product.
  */
-size_t pmx_prompt_attention_workspace_bytes(int64_t Tq, int32_t B, int32_t num_heads, int32_t num_kv_heads,
-                                            int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype);
-int pmx_prompt_attention(const void* query, const void* key, const void* value, const int64_t* seqstarts,
-                         const int64_t* kvstarts, const int64_t* prefix_lens, const float* alibi_slopes, void* out,
-                         int64_t Tq, int64_t Tk, int32_t B, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                         int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
-                         int64_t v_token_stride, int64_t v_head_stride, int64_t max_seqlen, int64_t max_kvlen,
-                         int32_t is_causal, float scale, float logit_cap, int32_t dtype, void* workspace,
-                         size_t workspace_bytes, void* stream);
+typedef struct pmx_prompt_attention_args {
+  const void *query, *key, *value;      /* [tokens, num_heads, head_dim], [keys, num_kv_heads, head_dim] */
+  const int64_t *seqstarts, *kvstarts, *prefix_lens;
+  const float* alibi_slopes;
+  void *out, *workspace;                /* out dense */
+  int64_t tokens, keys, sequences, num_heads, num_kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t max_seqlen, max_kvlen, is_causal, dtype, workspace_bytes;
+  double scale, logit_cap;
+} pmx_prompt_attention_args;
+/* bytes of workspace, 16-byte aligned, for either attention; 0: none is needed */
+size_t pmx_attention_workspace_bytes(int64_t tokens, int32_t sequences, int32_t num_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype);
+int pmx_prompt_attention(const pmx_prompt_attention_args* args, void* stream);
 
 /*
  * Attention of drafted tokens over the cache.  Sequence b brings seqstarts[b+1] - seqstarts[b] <= 64 drafted
@@ -429,17 +438,18 @@ int pmx_prompt_attention(const void* query, const void* key, const void* value, 
  * bit included, if it is to see itself).  Scores, empty rows, types and kernels as for pmx_prompt_attention;
  * cache strides as for pmx_decode_cache_attention, cache_rows rows in all (new rows outside are not stored).
  */
-size_t pmx_tree_cache_attention_workspace_bytes(int64_t Tq, int32_t B, int32_t num_heads, int32_t num_kv_heads,
-                                                int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype);
-int pmx_tree_cache_attention(const void* query, const void* current_key, const void* current_value, void* cache,
-                             const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
-                             const int64_t* tree_mask, void* out, int64_t Tq, int32_t B, int32_t num_heads,
-                             int32_t num_kv_heads, int32_t head_dim, int64_t q_token_stride, int64_t q_head_stride,
-                             int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                             int64_t v_head_stride, int64_t cache_rows, int64_t layer_offset, int64_t row_stride,
-                             int64_t kv_stride, int64_t head_stride, int64_t max_seqlen, int64_t max_kvlen, float scale,
-                             float logit_cap, int32_t dtype, void* workspace, size_t workspace_bytes,
-                             void* stream);
+typedef struct pmx_tree_attention_args {
+  const void *query, *current_key, *current_value;
+  void* cache;
+  const int64_t *seqstarts, *cachestarts, *start_pos, *tree_mask;
+  void *out, *workspace;
+  int64_t tokens, sequences, num_heads, num_kv_heads, head_dim;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t cache_rows, layer_offset, row_stride, kv_stride, head_stride;
+  int64_t max_seqlen, max_kvlen, dtype, workspace_bytes;
+  double scale, logit_cap;
+} pmx_tree_attention_args;
+int pmx_tree_cache_attention(const pmx_tree_attention_args* args, void* stream);
 /* Synchronises `stream`; PMX_ERR_DEVICE_CHECK (out = code, role, tile, CTA) if a bounded wait inside one of the two
  * attention kernels ran out on the current device since the last check (their results are then undefined), and
  * clears the record. */
@@ -454,11 +464,13 @@ int pmx_attention_check(int32_t out[4], void* stream);
  * cache element (row, layer, kv, head, d) lies at row*row_stride + layer*layer_stride + kv*kv_stride +
  * head*head_stride + d.
  */
-int pmx_compact_cache(void* cache, const int64_t* cachestarts, const int64_t* start_pos, const int64_t* accept_starts,
-                      const int64_t* accept_index, int64_t B, int64_t index_count, int32_t max_accept,
-                      int32_t num_layers, int32_t num_kv_heads, int32_t head_dim, int64_t cache_rows,
-                      int64_t row_stride, int64_t layer_stride, int64_t kv_stride, int64_t head_stride, int32_t dtype,
-                      void* stream);
+typedef struct pmx_compact_cache_args {
+  void* cache;
+  const int64_t *cachestarts, *start_pos, *accept_starts, *accept_index;
+  int64_t sequences, index_count, max_accept, num_layers, num_kv_heads, head_dim, cache_rows;
+  int64_t row_stride, layer_stride, kv_stride, head_stride, dtype;
+} pmx_compact_cache_args;
+int pmx_compact_cache(const pmx_compact_cache_args* args, void* stream);
 
 /* how pmx_moe_reduce_allreduce moves the partial results between the ranks */
 typedef enum pmx_allreduce_algorithm {

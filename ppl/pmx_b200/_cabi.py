@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -18,6 +19,14 @@ DTYPE_CODE = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 ABI_VERSION = 3
 EPILOGUE_NONE, EPILOGUE_SWIGLU = 0, 1
 GEMM_AUTO, GEMM_TC_TOKENS_M, GEMM_TC_WEIGHTS_M, GEMM_SIMT, GEMM_TC_TOKENS_M_PAIRED = 0, 1, 2, 3, 4
+
+
+# The argument structs of the attention block's entry points, packed member by member: all members are 8 bytes wide
+# (pointers and integers, then doubles), and one packed struct costs a call far less than thirty converted arguments.
+ROTARY_ARGS = struct.Struct("=22q2d")               # pmx_rotary_args
+PROMPT_ATTENTION_ARGS = struct.Struct("=26q2d")     # pmx_prompt_attention_args
+TREE_ATTENTION_ARGS = struct.Struct("=30q2d")       # pmx_tree_attention_args
+COMPACT_CACHE_ARGS = struct.Struct("=17q")          # pmx_compact_cache_args
 
 
 class GemmPlan(C.Structure):
@@ -80,18 +89,12 @@ def _load() -> C.CDLL:
         "pmx_decode_cache_attention_workspace_bytes": (sz, [i64, i32, i32, i32, i64]),
         "pmx_decode_cache_attention": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i64, i64, i64, i64, i64,
                                                  i32, vp, sz, vp]),
-        "pmx_rotary_embedding": (C.c_int, [vp, vp, vp, vp, f32, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i64, i64,
-                                           i64, i64, vp, i32, f32, i32, i32, vp]),
-        "pmx_prompt_attention_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64, i64, i32]),
-        "pmx_prompt_attention": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, i32, i64, i64, i64,
-                                           i64, i64, i64, i64, i64, i32, f32, f32, i32, vp, sz, vp]),
-        "pmx_tree_cache_attention_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64, i64, i32]),
-        "pmx_tree_cache_attention": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i64, i64,
-                                               i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, f32, f32, i32, vp,
-                                               sz, vp]),
+        "pmx_rotary_embedding": (C.c_int, [C.c_char_p, vp]),
+        "pmx_attention_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64, i64, i32]),
+        "pmx_prompt_attention": (C.c_int, [C.c_char_p, vp]),
+        "pmx_tree_cache_attention": (C.c_int, [C.c_char_p, vp]),
         "pmx_attention_check": (C.c_int, [C.POINTER(i32 * 4), vp]),
-        "pmx_compact_cache": (C.c_int, [vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, i32, i64, i64, i64, i64, i64, i32,
-                                        vp]),
+        "pmx_compact_cache": (C.c_int, [C.c_char_p, vp]),
         "pmx_moe_reduce_allreduce_buffer_bytes": (sz, [i64, i64, i32]),
         "pmx_moe_reduce_allreduce": (C.c_int, [vp, vp, vp, vp, i64, i32, i64, i32, C.POINTER(vp), i32, i32, sz,
                                                i32, i32, i64, vp]),

@@ -383,56 +383,24 @@ int pmx_decode_cache_attention(const void* query, const void* current_key, const
                                  dtype, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
-int pmx_rotary_embedding(const void* query, const void* key, const void* query_norm_weight, const void* key_norm_weight,
-                         float eps, void* query_out, void* key_out, const int64_t* seqstarts, const int64_t* start_pos,
-                         const int64_t* position_ids, int64_t T, int32_t B, int32_t num_heads, int32_t num_kv_heads,
-                         int32_t head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
-                         int64_t k_head_stride, const double* frequencies, int32_t rotary_dim, float factor,
-                         int32_t interleaved, int32_t dtype, void* stream) {
-  if (rotary_dim % 2) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: rotary_dim must be even");
-  return launch_rotary(query, key, query_norm_weight, key_norm_weight, eps, query_out, key_out, seqstarts, start_pos,
-                       position_ids, T, B, num_heads, num_kv_heads, head_dim, q_token_stride, q_head_stride,
-                       k_token_stride, k_head_stride, frequencies, rotary_dim / 2, factor, interleaved, dtype,
-                       (cudaStream_t)stream);
+int pmx_rotary_embedding(const pmx_rotary_args* args, void* stream) {
+  if (!args) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: null pointer");
+  return launch_rotary(*args, (cudaStream_t)stream);
 }
 
-size_t pmx_prompt_attention_workspace_bytes(int64_t Tq, int32_t B, int32_t num_heads, int32_t num_kv_heads,
-                                            int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype) {
-  return prompt_attention_workspace_bytes(Tq, B, num_heads, num_kv_heads, head_dim, max_seqlen, max_kvlen, dtype);
+size_t pmx_attention_workspace_bytes(int64_t tokens, int32_t sequences, int32_t num_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype) {
+  return attention_workspace_bytes(tokens, sequences, num_heads, num_kv_heads, head_dim, max_seqlen, max_kvlen, dtype);
 }
 
-int pmx_prompt_attention(const void* query, const void* key, const void* value, const int64_t* seqstarts,
-                         const int64_t* kvstarts, const int64_t* prefix_lens, const float* alibi_slopes, void* out,
-                         int64_t Tq, int64_t Tk, int32_t B, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                         int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
-                         int64_t v_token_stride, int64_t v_head_stride, int64_t max_seqlen, int64_t max_kvlen,
-                         int32_t is_causal, float scale, float logit_cap, int32_t dtype, void* workspace,
-                         size_t workspace_bytes, void* stream) {
-  const PromptAttention p{query, key, value, seqstarts, kvstarts, prefix_lens, alibi_slopes, out, Tq, Tk, B, num_heads,
-                          num_kv_heads, head_dim, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
-                          v_token_stride, v_head_stride, max_seqlen, max_kvlen, is_causal, scale, logit_cap, dtype};
-  return launch_prompt_attention(p, workspace, workspace_bytes, (cudaStream_t)stream);
+int pmx_prompt_attention(const pmx_prompt_attention_args* args, void* stream) {
+  if (!args) return fail(PMX_ERR_INVALID_ARGUMENT, "prompt_attention: null pointer");
+  return launch_prompt_attention(*args, (cudaStream_t)stream);
 }
 
-size_t pmx_tree_cache_attention_workspace_bytes(int64_t Tq, int32_t B, int32_t num_heads, int32_t num_kv_heads,
-                                                int32_t head_dim, int64_t max_seqlen, int64_t max_kvlen, int32_t dtype) {
-  return tree_attention_workspace_bytes(Tq, B, num_heads, num_kv_heads, head_dim, max_seqlen, max_kvlen, dtype);
-}
-
-int pmx_tree_cache_attention(const void* query, const void* current_key, const void* current_value, void* cache,
-                             const int64_t* seqstarts, const int64_t* cachestarts, const int64_t* start_pos,
-                             const int64_t* tree_mask, void* out, int64_t Tq, int32_t B, int32_t num_heads,
-                             int32_t num_kv_heads, int32_t head_dim, int64_t q_token_stride, int64_t q_head_stride,
-                             int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
-                             int64_t v_head_stride, int64_t cache_rows, int64_t layer_offset, int64_t row_stride,
-                             int64_t kv_stride, int64_t head_stride, int64_t max_seqlen, int64_t max_kvlen, float scale,
-                             float logit_cap, int32_t dtype, void* workspace, size_t workspace_bytes,
-                             void* stream) {
-  const TreeAttention p{query, current_key, current_value, cache, seqstarts, cachestarts, start_pos, tree_mask, out, Tq,
-                        B, num_heads, num_kv_heads, head_dim, q_token_stride, q_head_stride, k_token_stride,
-                        k_head_stride, v_token_stride, v_head_stride, cache_rows, layer_offset, row_stride, kv_stride,
-                        head_stride, max_seqlen, max_kvlen, scale, logit_cap, dtype};
-  return launch_tree_attention(p, workspace, workspace_bytes, (cudaStream_t)stream);
+int pmx_tree_cache_attention(const pmx_tree_attention_args* args, void* stream) {
+  if (!args) return fail(PMX_ERR_INVALID_ARGUMENT, "tree_cache_attention: null pointer");
+  return launch_tree_attention(*args, (cudaStream_t)stream);
 }
 
 int pmx_attention_check(int32_t out[4], void* stream) {
@@ -440,13 +408,9 @@ int pmx_attention_check(int32_t out[4], void* stream) {
   return attention_check(out, (cudaStream_t)stream);
 }
 
-int pmx_compact_cache(void* cache, const int64_t* cachestarts, const int64_t* start_pos, const int64_t* accept_starts,
-                      const int64_t* accept_index, int64_t B, int64_t index_count, int32_t max_accept,
-                      int32_t num_layers, int32_t num_kv_heads, int32_t head_dim, int64_t cache_rows, int64_t row_stride,
-                      int64_t layer_stride, int64_t kv_stride, int64_t head_stride, int32_t dtype, void* stream) {
-  return launch_compact_cache(cache, cachestarts, start_pos, accept_starts, accept_index, B, index_count, max_accept,
-                              num_layers, num_kv_heads, head_dim, cache_rows, row_stride, layer_stride, kv_stride,
-                              head_stride, dtype, (cudaStream_t)stream);
+int pmx_compact_cache(const pmx_compact_cache_args* args, void* stream) {
+  if (!args) return fail(PMX_ERR_INVALID_ARGUMENT, "compact_cache: null pointer");
+  return launch_compact_cache(*args, (cudaStream_t)stream);
 }
 
 size_t pmx_moe_reduce_allreduce_buffer_bytes(int64_t T, int64_t N, int32_t dtype) {

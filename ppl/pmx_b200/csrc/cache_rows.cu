@@ -54,37 +54,38 @@ __global__ void __launch_bounds__(128) compact_cache_kernel(const CompactArgs a)
 
 }  // namespace
 
-int launch_compact_cache(void* cache, const int64_t* cachestarts, const int64_t* start_pos, const int64_t* accept_starts,
-                         const int64_t* accept_index, int64_t B, int64_t index_count, int max_accept, int layers,
-                         int heads, int D, int64_t rows, int64_t row_stride, int64_t layer_stride, int64_t kv_stride,
-                         int64_t head_stride, int dtype, cudaStream_t s) {
-  if (!cache || !cachestarts || !start_pos || !accept_starts || !accept_index)
+int launch_compact_cache(const pmx_compact_cache_args& p, cudaStream_t s) {
+  if (!p.cache || !p.cachestarts || !p.start_pos || !p.accept_starts || !p.accept_index)
     return fail(PMX_ERR_INVALID_ARGUMENT, "compact_cache: null pointer");
-  if (B <= 0 || layers <= 0 || heads <= 0 || D <= 0 || rows <= 0 || max_accept <= 0 || index_count <= 0)
+  if (p.sequences <= 0 || p.num_layers <= 0 || p.num_kv_heads <= 0 || p.head_dim <= 0 || p.cache_rows <= 0 ||
+      p.max_accept <= 0 || p.index_count <= 0)
     return fail(PMX_ERR_INVALID_ARGUMENT, "compact_cache: sizes must be positive");
-  if (max_accept > 64) return fail(PMX_ERR_UNSUPPORTED, "compact_cache: at most 64 accepted rows a sequence");
-  if (B > 65535) return fail(PMX_ERR_UNSUPPORTED, "compact_cache: too many sequences");
+  if (p.max_accept > 64) return fail(PMX_ERR_UNSUPPORTED, "compact_cache: at most 64 accepted rows a sequence");
+  if (p.sequences > 65535 || p.num_layers > (1 << 20) || p.num_kv_heads > (1 << 20) || p.head_dim > (1 << 20))
+    return fail(PMX_ERR_UNSUPPORTED, "compact_cache: sizes beyond what the kernel indexes");
+  const int max_accept = (int)p.max_accept;
   int e;
-  switch (dtype) {
+  switch (p.dtype) {
     case PMX_DTYPE_F16: case PMX_DTYPE_BF16: e = 2; break;
     case PMX_DTYPE_F32: e = 4; break;
-    default: return fail(PMX_ERR_UNSUPPORTED, "compact_cache: unknown dtype %d", dtype);
+    default: return fail(PMX_ERR_UNSUPPORTED, "compact_cache: unknown dtype %d", (int)p.dtype);
   }
   // the widest vector that every head row begins on and divides into; 64 rows need the registers
   // that 16-byte vectors would take for 32
-  const uint64_t grain = (uint64_t)(row_stride | layer_stride | kv_stride | head_stride | D) * e | reinterpret_cast<uintptr_t>(cache);
+  const uint64_t grain = (uint64_t)(p.row_stride | p.layer_stride | p.kv_stride | p.head_stride | p.head_dim) * e |
+                         reinterpret_cast<uintptr_t>(p.cache);
   int vec = grain % 16 == 0 ? 16 : grain % 8 == 0 ? 8 : grain % 4 == 0 ? 4 : 2;
   if (max_accept > 32 && vec > 8) vec = 8;
   CompactArgs a{};
-  a.cache = (char*)cache;
-  a.cachestarts = cachestarts; a.start_pos = start_pos; a.accept_starts = accept_starts; a.accept_index = accept_index;
-  a.rows = rows; a.index_count = index_count;
-  a.row_bytes = row_stride * e; a.layer_bytes = layer_stride * e; a.kv_bytes = kv_stride * e; a.head_bytes = head_stride * e;
-  a.layers = layers; a.heads = heads; a.chunks = D * e / vec;
-  const int64_t cols = (int64_t)layers * 2 * heads * a.chunks;
+  a.cache = (char*)p.cache;
+  a.cachestarts = p.cachestarts; a.start_pos = p.start_pos; a.accept_starts = p.accept_starts; a.accept_index = p.accept_index;
+  a.rows = p.cache_rows; a.index_count = p.index_count;
+  a.row_bytes = p.row_stride * e; a.layer_bytes = p.layer_stride * e; a.kv_bytes = p.kv_stride * e; a.head_bytes = p.head_stride * e;
+  a.layers = (int)p.num_layers; a.heads = (int)p.num_kv_heads; a.chunks = (int)p.head_dim * e / vec;
+  const int64_t cols = p.num_layers * 2 * p.num_kv_heads * a.chunks;
   const int64_t blocks = ceil_div(cols, 128);
   if (blocks > 0x7FFFFFFFll) return fail(PMX_ERR_UNSUPPORTED, "compact_cache: cache too wide");
-  const dim3 grid((unsigned)blocks, (unsigned)B), block(128);
+  const dim3 grid((unsigned)blocks, (unsigned)p.sequences), block(128);
   if (vec == 16) {
     if (max_accept <= 8) return launch_pdl_k(compact_cache_kernel<uint4, 8>, grid, block, 0, s, a);
     if (max_accept <= 16) return launch_pdl_k(compact_cache_kernel<uint4, 16>, grid, block, 0, s, a);

@@ -162,46 +162,12 @@ int launch_decode_attention(const void* q, const void* k_cur, const void* v_cur,
                             int Hkv, int D, int64_t layer_off, int64_t row_stride, int64_t kv_stride,
                             int64_t head_stride, int64_t max_kvlen, int dtype, void* ws, size_t ws_bytes,
                             cudaStream_t s);
-int launch_rotary(const void* q, const void* k, const void* qw, const void* kw, float eps, void* qo, void* ko,
-                  const int64_t* seqstarts, const int64_t* start_pos, const int64_t* position_ids, int64_t T, int B,
-                  int Hq, int Hkv, int D, int64_t q_tok, int64_t q_head, int64_t k_tok, int64_t k_head,
-                  const double* frequencies, int pairs, float factor, int interleaved, int dtype, cudaStream_t s);
-int launch_compact_cache(void* cache, const int64_t* cachestarts, const int64_t* start_pos, const int64_t* accept_starts,
-                         const int64_t* accept_index, int64_t B, int64_t index_count, int max_accept, int layers,
-                         int heads, int D, int64_t rows, int64_t row_stride, int64_t layer_stride, int64_t kv_stride,
-                         int64_t head_stride, int dtype, cudaStream_t s);
-
-// pmx_prompt_attention and pmx_tree_cache_attention as declared in pmx_moe.h
-struct PromptAttention {
-  const void *q, *k, *v;
-  const int64_t *seqstarts, *kvstarts, *prefix;
-  const float* slopes;
-  void* out;
-  int64_t Tq, Tk;
-  int B, Hq, Hkv, D;
-  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, max_seqlen, max_kvlen;
-  int causal;
-  float scale, cap;
-  int dtype;
-};
-struct TreeAttention {
-  const void *q, *k, *v;
-  void* cache;
-  const int64_t *seqstarts, *cachestarts, *start_pos, *tree_mask;
-  void* out;
-  int64_t Tq;
-  int B, Hq, Hkv, D;
-  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, rows, layer_off, row_stride, kv_stride, head_stride, max_seqlen,
-      max_kvlen;
-  float scale, cap;
-  int dtype;
-};
-size_t prompt_attention_workspace_bytes(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, int64_t max_kvlen,
-                                        int dtype);
-size_t tree_attention_workspace_bytes(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, int64_t max_kvlen,
-                                      int dtype);
-int launch_prompt_attention(const PromptAttention& p, void* ws, size_t ws_bytes, cudaStream_t s);
-int launch_tree_attention(const TreeAttention& p, void* ws, size_t ws_bytes, cudaStream_t s);
+int launch_rotary(const pmx_rotary_args& p, cudaStream_t s);
+int launch_compact_cache(const pmx_compact_cache_args& p, cudaStream_t s);
+size_t attention_workspace_bytes(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_seqlen,
+                                 int64_t max_kvlen, int dtype);
+int launch_prompt_attention(const pmx_prompt_attention_args& p, cudaStream_t s);
+int launch_tree_attention(const pmx_tree_attention_args& p, cudaStream_t s);
 int attention_check(int out[4], cudaStream_t s);
 int launch_zero_outside(void* y, const int64_t* off, int64_t M, int64_t n_out, int E, int dtype,
                         cudaStream_t s);

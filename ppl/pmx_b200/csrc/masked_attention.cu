@@ -199,18 +199,6 @@ namespace tc {
 #include "masked_attention_tc.cuh"
 }
 
-int check_common(const AttnArgs& a, int dtype, const char* name) {
-  if (a.Tq <= 0 || a.B <= 0 || a.Hq <= 0 || a.Hkv <= 0 || a.D <= 0 || a.max_seqlen <= 0 || a.Hq % a.Hkv)
-    return fail(PMX_ERR_INVALID_ARGUMENT, "%s: sizes must be positive and num_heads a multiple of num_kv_heads (tokens=%lld B=%d heads=%d/%d)", name, (long long)a.Tq, a.B, a.Hq, a.Hkv);
-  if (a.D > kMaxHeadDim) return fail(PMX_ERR_UNSUPPORTED, "%s: head_dim %d (at most %d)", name, a.D, kMaxHeadDim);
-  if (a.B > 65534 || a.Hkv > 65535) return fail(PMX_ERR_UNSUPPORTED, "%s: too many sequences or heads", name);
-  if (dtype != PMX_DTYPE_F16 && dtype != PMX_DTYPE_BF16 && dtype != PMX_DTYPE_F32)
-    return fail(PMX_ERR_UNSUPPORTED, "%s: unknown dtype %d", name, dtype);
-  if (!(a.scale > 0.f) || a.scale > 3e38f) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", name);
-  if (!(a.cap >= 0.f) || a.cap > 3e38f) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: logit_cap must be finite and not negative", name);
-  return PMX_OK;
-}
-
 }  // namespace
 
 int attention_check(int out[4], cudaStream_t s) {
@@ -224,59 +212,62 @@ int attention_check(int out[4], cudaStream_t s) {
   return fail(PMX_ERR_DEVICE_CHECK, "attention: a wait inside a kernel ran out (role %d, tile %d, CTA %d)", out[1], out[2], out[3]);
 }
 
-size_t prompt_attention_workspace_bytes(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, int64_t max_kvlen,
-                                        int dtype) {
+size_t attention_workspace_bytes(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_seqlen,
+                                 int64_t max_kvlen, int dtype) {
   return tc::tc_workspace(tc::plan_tc(Tq, B, Hq, Hkv, D, max_seqlen, max_kvlen, dtype), Tq, Hq, D);
 }
 
-size_t tree_attention_workspace_bytes(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, int64_t max_kvlen,
-                                        int dtype) {
-  return tc::tc_workspace(tc::plan_tc(Tq, B, Hq, Hkv, D, max_seqlen, max_kvlen, dtype), Tq, Hq, D);
-}
-
-int launch_prompt_attention(const PromptAttention& p, void* ws, size_t ws_bytes, cudaStream_t s) {
-  const char* name = "prompt_attention";
-  if (!p.q || !p.k || !p.v || !p.out || !p.seqstarts || !p.kvstarts) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
-  if (p.Tk <= 0 || p.max_kvlen <= 0) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: there must be keys", name);
-  AttnArgs a{};
-  a.q = p.q; a.q_tok = p.q_tok; a.q_head = p.q_head;
-  a.past = KvRows{p.k, p.v, p.k_tok, p.k_head, p.v_tok, p.v_head, p.Tk};
-  a.seqstarts = p.seqstarts; a.kvstarts = p.kvstarts; a.prefix = p.prefix; a.slopes = p.slopes;
-  a.out = p.out; a.Tq = p.Tq; a.B = p.B; a.Hq = p.Hq; a.Hkv = p.Hkv; a.D = p.D;
-  a.max_seqlen = (int)(p.max_seqlen < p.Tq ? p.max_seqlen : p.Tq);
-  a.causal = p.causal; a.scale = p.scale; a.cap = p.cap;
-  const int st = check_common(a, p.dtype, name);
-  if (st != PMX_OK) return st;
-  const size_t need = prompt_attention_workspace_bytes(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype);
-  if (!ws || ws_bytes < need) return fail(PMX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", name, need, ws_bytes);
+// what the two operators share once their own arguments are in place
+template <typename P>
+int run_attention(AttnArgs& a, const P& p, const char* name, cudaStream_t s) {
+  if (p.tokens <= 0 || p.sequences <= 0 || p.num_heads <= 0 || p.num_kv_heads <= 0 || p.head_dim <= 0 ||
+      p.max_seqlen <= 0 || p.max_kvlen <= 0 || a.past.rows <= 0 || p.num_heads % p.num_kv_heads)
+    return fail(PMX_ERR_INVALID_ARGUMENT, "%s: sizes must be positive and num_heads a multiple of num_kv_heads (tokens=%lld sequences=%lld heads=%lld/%lld)", name, (long long)p.tokens, (long long)p.sequences, (long long)p.num_heads, (long long)p.num_kv_heads);
+  if (p.head_dim > kMaxHeadDim) return fail(PMX_ERR_UNSUPPORTED, "%s: head_dim %lld (at most %d)", name, (long long)p.head_dim, kMaxHeadDim);
+  if (p.sequences > (1 << 20) || p.num_heads > (1 << 16) || p.tokens > (1ll << 40)) return fail(PMX_ERR_UNSUPPORTED, "%s: too many sequences, heads or tokens", name);
+  if (p.dtype != PMX_DTYPE_F16 && p.dtype != PMX_DTYPE_BF16 && p.dtype != PMX_DTYPE_F32)
+    return fail(PMX_ERR_UNSUPPORTED, "%s: unknown dtype %d", name, (int)p.dtype);
+  a.q = p.query; a.q_tok = p.q_token_stride; a.q_head = p.q_head_stride;
+  a.seqstarts = p.seqstarts;
+  a.out = p.out; a.Tq = p.tokens; a.B = (int)p.sequences; a.Hq = (int)p.num_heads; a.Hkv = (int)p.num_kv_heads;
+  a.D = (int)p.head_dim;
+  const int64_t most = p.max_seqlen < p.tokens ? p.max_seqlen : p.tokens;
+  a.max_seqlen = (int)(most < 0x7FFFFFFF ? most : 0x7FFFFFFF);
+  a.scale = (float)p.scale; a.cap = (float)p.logit_cap;
+  if (!(a.scale > 0.f) || a.scale > 3e38f) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", name);
+  if (!(a.cap >= 0.f) || a.cap > 3e38f) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: logit_cap must be finite and not negative", name);
+  const tc::TcPlan plan = tc::plan_tc(p.tokens, p.sequences, p.num_heads, p.num_kv_heads, p.head_dim, p.max_seqlen, p.max_kvlen, (int)p.dtype);
+  const size_t need = tc::tc_workspace(plan, p.tokens, p.num_heads, p.head_dim);
+  if (need && (!p.workspace || p.workspace_bytes < (int64_t)need))
+    return fail(PMX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %lld given", name, need, (long long)p.workspace_bytes);
+  if (need && !aligned16(p.workspace)) return fail(PMX_ERR_ALIGNMENT, "%s: the workspace must be 16-byte aligned", name);
   bool done;
-  const int tc_status = tc::launch_tc(a, tc::plan_tc(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype), p.dtype, name, ws, s, &done);
-  return done ? tc_status : launch_rows(a, p.dtype, name, s);
+  const int st = tc::launch_tc(a, plan, (int)p.dtype, name, p.workspace, s, &done);
+  return done ? st : launch_rows(a, (int)p.dtype, name, s);
 }
 
-int launch_tree_attention(const TreeAttention& p, void* ws, size_t ws_bytes, cudaStream_t s) {
+int launch_prompt_attention(const pmx_prompt_attention_args& p, cudaStream_t s) {
+  const char* name = "prompt_attention";
+  if (!p.query || !p.key || !p.value || !p.out || !p.seqstarts || !p.kvstarts) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
+  AttnArgs a{};
+  a.past = KvRows{p.key, p.value, p.k_token_stride, p.k_head_stride, p.v_token_stride, p.v_head_stride, p.keys};
+  a.kvstarts = p.kvstarts; a.prefix = p.prefix_lens; a.slopes = p.alibi_slopes;
+  a.causal = p.is_causal != 0;
+  return run_attention(a, p, name, s);
+}
+
+int launch_tree_attention(const pmx_tree_attention_args& p, cudaStream_t s) {
   const char* name = "tree_cache_attention";
-  if (!p.q || !p.k || !p.v || !p.out || !p.cache || !p.seqstarts || !p.cachestarts || !p.start_pos || !p.tree_mask)
+  if (!p.query || !p.current_key || !p.current_value || !p.out || !p.cache || !p.seqstarts || !p.cachestarts || !p.start_pos || !p.tree_mask)
     return fail(PMX_ERR_INVALID_ARGUMENT, "%s: null pointer", name);
-  if (p.rows <= 0 || p.max_kvlen <= 0) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: the cache must have rows", name);
   if (p.max_seqlen > kTreeLimit) return fail(PMX_ERR_UNSUPPORTED, "%s: at most %d drafted tokens a sequence", name, kTreeLimit);
   const int e = p.dtype == PMX_DTYPE_F32 ? 4 : 2;
-  char* layer = (char*)p.cache + p.layer_off * e;
+  char* layer = (char*)p.cache + p.layer_offset * e;
   AttnArgs a{};
-  a.q = p.q; a.q_tok = p.q_tok; a.q_head = p.q_head;
-  a.past = KvRows{layer, layer + p.kv_stride * e, p.row_stride, p.head_stride, p.row_stride, p.head_stride, p.rows};
-  a.cur = KvRows{p.k, p.v, p.k_tok, p.k_head, p.v_tok, p.v_head, p.Tq};
-  a.seqstarts = p.seqstarts; a.cachestarts = p.cachestarts; a.start_pos = p.start_pos; a.tree_mask = p.tree_mask;
-  a.out = p.out; a.Tq = p.Tq; a.B = p.B; a.Hq = p.Hq; a.Hkv = p.Hkv; a.D = p.D;
-  a.max_seqlen = (int)(p.max_seqlen < p.Tq ? p.max_seqlen : p.Tq);
-  a.causal = 0; a.scale = p.scale; a.cap = p.cap;
-  const int st = check_common(a, p.dtype, name);
-  if (st != PMX_OK) return st;
-  const size_t need = tree_attention_workspace_bytes(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype);
-  if (!ws || ws_bytes < need) return fail(PMX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", name, need, ws_bytes);
-  bool done;
-  const int tc_status = tc::launch_tc(a, tc::plan_tc(p.Tq, p.B, p.Hq, p.Hkv, p.D, p.max_seqlen, p.max_kvlen, p.dtype), p.dtype, name, ws, s, &done);
-  return done ? tc_status : launch_rows(a, p.dtype, name, s);
+  a.past = KvRows{layer, layer + p.kv_stride * e, p.row_stride, p.head_stride, p.row_stride, p.head_stride, p.cache_rows};
+  a.cur = KvRows{p.current_key, p.current_value, p.k_token_stride, p.k_head_stride, p.v_token_stride, p.v_head_stride, p.tokens};
+  a.cachestarts = p.cachestarts; a.start_pos = p.start_pos; a.tree_mask = p.tree_mask;
+  return run_attention(a, p, name, s);
 }
 
 }  // namespace pmx

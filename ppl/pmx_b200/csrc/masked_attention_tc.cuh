@@ -741,18 +741,19 @@ struct TcPlan {
 };
 
 // Everything that sizes the workspace and the grid follows from shapes and host lengths alone.
-TcPlan plan_tc(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, int64_t max_kvlen, int dtype) {
+TcPlan plan_tc(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_seqlen, int64_t max_kvlen, int dtype) {
   TcPlan pl{};
-  if ((dtype != PMX_DTYPE_F16 && dtype != PMX_DTYPE_BF16) || D % 8 || D > 128 || Hkv <= 0 || Hq % Hkv || Hq / Hkv > kTile)
+  if ((dtype != PMX_DTYPE_F16 && dtype != PMX_DTYPE_BF16) || D % 8 || D > 128 || Hkv <= 0 ||
+      Hq % Hkv || Hq / Hkv > kTile)
     return pl;
-  if (Tq <= 0 || B <= 0 || max_seqlen <= 0 || max_kvlen <= 0 || Tq >= (1ll << 31)) return pl;
+  if (Tq <= 0 || B <= 0 || Hq <= 0 || D <= 0 || max_seqlen <= 0 || max_kvlen <= 0 || Tq >= (1ll << 31)) return pl;
   if (max_seqlen > Tq) max_seqlen = Tq;
-  pl.group = Hq / Hkv;
+  pl.group = (int)(Hq / Hkv);
   pl.tokens = kTile / pl.group;
   pl.pair = max_seqlen > pl.tokens;
   const int64_t blocks = ceil_div(max_seqlen, pl.pair ? 2 * pl.tokens : pl.tokens);
   const int64_t ctas = blocks * B * Hkv, tiles = ceil_div(max_kvlen, kTile);
-  if (ctas > (1 << 24)) return pl;
+  if (ctas > (1 << 24) || B > (1 << 20)) return pl;
   pl.row_blocks = (int)blocks;
   // Split the keys while that fills SMs that would idle, with at least 4 key tiles a CTA: below that the start of a
   // CTA and the merge cost more than the shorter walk gains.
@@ -763,8 +764,8 @@ TcPlan plan_tc(int64_t Tq, int B, int Hq, int Hkv, int D, int64_t max_seqlen, in
   return pl;
 }
 
-size_t tc_workspace(const TcPlan& pl, int64_t Tq, int Hq, int D) {
-  if (!pl.use || pl.splits == 1) return 16;
+size_t tc_workspace(const TcPlan& pl, int64_t Tq, int64_t Hq, int64_t D) {
+  if (!pl.use || pl.splits == 1) return 0;
   return (size_t)pl.splits * Tq * Hq * ((size_t)D * sizeof(float) + sizeof(float2));
 }
 

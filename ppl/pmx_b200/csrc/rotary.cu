@@ -258,30 +258,35 @@ int launch_rotary_t(RotaryArgs& a, bool norm, bool interleaved, cudaStream_t s) 
 
 }  // namespace
 
-int launch_rotary(const void* q, const void* k, const void* qw, const void* kw, float eps, void* qo, void* ko,
-                  const int64_t* seqstarts, const int64_t* start_pos, const int64_t* position_ids, int64_t T, int B,
-                  int Hq, int Hkv, int D, int64_t q_tok, int64_t q_head, int64_t k_tok, int64_t k_head,
-                  const double* frequencies, int pairs, float factor, int interleaved, int dtype, cudaStream_t s) {
-  if (!q || !qo || !frequencies) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: null pointer");
-  if (T <= 0 || Hq <= 0 || D <= 0 || Hkv < 0) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: T, heads and head_dim must be positive");
-  if ((Hkv > 0) != (k != nullptr) || (k && !ko)) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: key, its output and num_kv_heads go together");
-  if (!position_ids && (!seqstarts || !start_pos || B <= 0))
+int launch_rotary(const pmx_rotary_args& p, cudaStream_t s) {
+  if (!p.query || !p.query_out || !p.frequencies) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: null pointer");
+  if (p.tokens <= 0 || p.num_heads <= 0 || p.head_dim <= 0 || p.num_kv_heads < 0)
+    return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: tokens, heads and head_dim must be positive");
+  if (p.num_heads > (1 << 20) || p.num_kv_heads > (1 << 20) || p.head_dim > (1 << 20) || p.sequences > (1ll << 30))
+    return fail(PMX_ERR_UNSUPPORTED, "rotary_embedding: sizes beyond what the kernels index");
+  if ((p.num_kv_heads > 0) != (p.key != nullptr) || (p.key && !p.key_out))
+    return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: key, its output and num_kv_heads go together");
+  if (!p.position_ids && (!p.seqstarts || !p.start_pos || p.sequences <= 0))
     return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: positions come from position_ids or from seqstarts and start_pos");
-  if (pairs <= 0 || 2 * pairs > D) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: rotary_dim must be even, positive and at most head_dim");
-  if (pairs > kRotMaxPairs) return fail(PMX_ERR_UNSUPPORTED, "rotary_embedding: rotary_dim of at most %d", 2 * kRotMaxPairs);
-  if ((kw != nullptr) != (qw != nullptr && k != nullptr)) return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: norm weights are given for query and key, or for neither");
+  if (p.rotary_dim <= 0 || p.rotary_dim % 2 || p.rotary_dim > p.head_dim)
+    return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: rotary_dim must be even, positive and at most head_dim");
+  if (p.rotary_dim > 2 * kRotMaxPairs) return fail(PMX_ERR_UNSUPPORTED, "rotary_embedding: rotary_dim of at most %d", 2 * kRotMaxPairs);
+  if ((p.key_norm_weight != nullptr) != (p.query_norm_weight != nullptr && p.key != nullptr))
+    return fail(PMX_ERR_INVALID_ARGUMENT, "rotary_embedding: norm weights are given for query and key, or for neither");
   RotaryArgs a{};
-  for (int i = 0; i < pairs; ++i) a.turns[i] = frequencies[i] * 0.15915494309189533577;   // 1 / (2 pi)
-  a.q = q; a.k = k; a.qw = qw; a.kw = kw; a.qo = qo; a.ko = ko;
-  a.q_tok = q_tok; a.q_head = q_head; a.k_tok = k_tok; a.k_head = k_head;
-  a.seqstarts = seqstarts; a.start_pos = start_pos; a.position_ids = position_ids;
-  a.T = T; a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.D = D; a.pairs = pairs; a.eps = eps; a.factor = factor;
-  switch (dtype) {
-    case PMX_DTYPE_F16: return launch_rotary_t<__half>(a, qw != nullptr, interleaved != 0, s);
-    case PMX_DTYPE_BF16: return launch_rotary_t<__nv_bfloat16>(a, qw != nullptr, interleaved != 0, s);
-    case PMX_DTYPE_F32: return launch_rotary_t<float>(a, qw != nullptr, interleaved != 0, s);
+  a.pairs = (int)p.rotary_dim / 2;
+  for (int i = 0; i < a.pairs; ++i) a.turns[i] = p.frequencies[i] * 0.15915494309189533577;   // 1 / (2 pi)
+  a.q = p.query; a.k = p.key; a.qw = p.query_norm_weight; a.kw = p.key_norm_weight; a.qo = p.query_out; a.ko = p.key_out;
+  a.q_tok = p.q_token_stride; a.q_head = p.q_head_stride; a.k_tok = p.k_token_stride; a.k_head = p.k_head_stride;
+  a.seqstarts = p.seqstarts; a.start_pos = p.start_pos; a.position_ids = p.position_ids;
+  a.T = p.tokens; a.B = (int)p.sequences; a.Hq = (int)p.num_heads; a.Hkv = (int)p.num_kv_heads; a.D = (int)p.head_dim;
+  a.eps = (float)p.eps; a.factor = (float)p.factor;
+  switch (p.dtype) {
+    case PMX_DTYPE_F16: return launch_rotary_t<__half>(a, a.qw != nullptr, p.interleaved != 0, s);
+    case PMX_DTYPE_BF16: return launch_rotary_t<__nv_bfloat16>(a, a.qw != nullptr, p.interleaved != 0, s);
+    case PMX_DTYPE_F32: return launch_rotary_t<float>(a, a.qw != nullptr, p.interleaved != 0, s);
   }
-  return fail(PMX_ERR_UNSUPPORTED, "rotary_embedding: unknown dtype %d", dtype);
+  return fail(PMX_ERR_UNSUPPORTED, "rotary_embedding: unknown dtype %d", (int)p.dtype);
 }
 
 }  // namespace pmx

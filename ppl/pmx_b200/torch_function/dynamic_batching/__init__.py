@@ -20,6 +20,7 @@ import torch
 
 from ..._cabi import lib, check, ptr, stream_of, workspace, DTYPE_CODE
 from ..moe import _require_cuda
+from ._common import cache_strides
 
 
 def set_decode_attention_kernel(kind: str) -> str:
@@ -28,33 +29,6 @@ def set_decode_attention_kernel(kind: str) -> str:
     Process-wide; returns the previous choice."""
     names = ("mma", "simt")
     return names[lib.pmx_decode_cache_attention_set_kernel(names.index(kind))]
-
-
-def cache_strides(cache: torch.Tensor, cache_layout: int, num_layer: int, layer_idx: int):
-    """-> (layer_offset, row_stride, kv_stride, head_stride, total_rows) in elements for the
-    four cache layouts of cache_mode 0 (Pipeline.py:80-89 of the Mixtral model):
-      0: [rows, layers, 2, heads, d]   1: [layers, rows, 2, heads, d]
-      2: [layers, 2, rows, heads, d]   3: [layers, 2, heads, rows, d]"""
-    if cache.dim() != 5 or not cache.is_contiguous():
-        raise ValueError("the cache must be a contiguous 5-d tensor")
-    d = cache.shape[-1]
-    if cache_layout == 0:
-        rows, layers, two, heads, _ = cache.shape
-        st = (layer_idx * 2 * heads * d, layers * 2 * heads * d, heads * d, d)
-    elif cache_layout == 1:
-        layers, rows, two, heads, _ = cache.shape
-        st = (layer_idx * rows * 2 * heads * d, 2 * heads * d, heads * d, d)
-    elif cache_layout == 2:
-        layers, two, rows, heads, _ = cache.shape
-        st = (layer_idx * 2 * rows * heads * d, heads * d, rows * heads * d, d)
-    elif cache_layout == 3:
-        layers, two, heads, rows, _ = cache.shape
-        st = (layer_idx * 2 * heads * rows * d, d, heads * rows * d, rows * d)
-    else:
-        raise ValueError(f"unsupported cache_layout: {cache_layout}")
-    if two != 2 or layers != num_layer or not 0 <= layer_idx < layers:
-        raise ValueError(f"cache shape {tuple(cache.shape)} does not fit layout {cache_layout} with {num_layer} layers")
-    return st + (rows,)
 
 
 class MultiHeadCacheAttention(torch.autograd.Function):

@@ -3,8 +3,8 @@ from __future__ import annotations
 
 import torch
 
-from ..._cabi import lib, check, stream_of, DTYPE_CODE
-from ._common import host_int, index, on_device, same_device
+from ..._cabi import lib, check, COMPACT_CACHE_ARGS, DTYPE_CODE
+from ._common import cache_strides, host_int, index, on_device, raw_stream, same_device
 
 
 def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: torch.Tensor, accept_starts: torch.Tensor,
@@ -17,10 +17,11 @@ def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: tor
     written, so the indices may come in any order and repeat; a negative index leaves its row alone.  The caller's next
     start_pos is start_pos + the number accepted.  Rows of different sequences must not overlap."""
     name = "compact_cache"
-    from . import cache_strides
-    dev = cache.device
-    same_device(name, dev if cache.is_cuda else torch.device("cuda"), cache=cache, cachestarts=cachestarts,
-                start_pos=start_pos, accept_starts=accept_starts, accept_index=accept_index)
+    dev = cache.get_device()
+    for t in (cache, cachestarts, start_pos, accept_starts, accept_index):
+        if dev < 0 or t.get_device() != dev:
+            same_device(name, dev, cache=cache, cachestarts=cachestarts, start_pos=start_pos,
+                        accept_starts=accept_starts, accept_index=accept_index)
     code = DTYPE_CODE.get(cache.dtype)
     if code is None:
         raise TypeError(f"{name}: dtype {cache.dtype} is not supported (float16, bfloat16, float32)")
@@ -41,8 +42,8 @@ def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: tor
     if accept_index.numel() == 0 or cache.numel() == 0:
         return cache
     with on_device(dev):
-        check(lib.pmx_compact_cache(cache.data_ptr(), cachestarts.data_ptr(), start_pos.data_ptr(),
-                                    accept_starts.data_ptr(), accept_index.data_ptr(), B, accept_index.numel(),
-                                    max_accept, num_layer, kv_heads, cache.shape[-1], rows, row_stride, layer_stride,
-                                    kv_stride, head_stride, code, stream_of(cache)))
+        check(lib.pmx_compact_cache(COMPACT_CACHE_ARGS.pack(
+            cache.data_ptr(), cachestarts.data_ptr(), start_pos.data_ptr(), accept_starts.data_ptr(),
+            accept_index.data_ptr(), B, accept_index.numel(), max_accept, num_layer, kv_heads, cache.shape[-1], rows,
+            row_stride, layer_stride, kv_stride, head_stride, code), raw_stream(dev)))
     return cache

@@ -8,13 +8,15 @@ merge where a long key axis is split because there are few rows.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional
 
 import torch
 
-from ..._cabi import lib, check, stream_of, workspace, DTYPE_CODE
-from ._common import heads, host_int, index, on_device, same_device, wants_grad
+from ..._cabi import lib, check, workspace, DTYPE_CODE, PROMPT_ATTENTION_ARGS, TREE_ATTENTION_ARGS
+from ._common import (cache_strides, exporting, heads, host_int, index, on_device, raw_stream, same_device,
+                      wants_grad)
 
 
 
@@ -37,23 +39,28 @@ def _numbers(name: str, num_heads: int, kv_heads: int, head_dim: int, scale, log
     return scale
 
 
+# bytes of workspace by sizes; the GPU (they depend on its number of SMs) is the process's kind of GPU
+_workspace_bytes = functools.lru_cache(maxsize=1024)(lib.pmx_attention_workspace_bytes)
+
+
 def attention_check(device=None) -> None:
     """Synchronises the current stream of the device and raises PmxError (status -6) if a bounded wait inside
     prompt_attention or tree_cache_attention ran out since the last check (their results are then undefined)."""
     dev = torch.device("cuda" if device is None else device)
-    if dev.index is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
+    dev = torch.cuda.current_device() if dev.index is None else dev.index
     out = (C.c_int32 * 4)()
     with on_device(dev):
-        check(lib.pmx_attention_check(C.byref(out), torch.cuda.current_stream(dev).cuda_stream))
+        check(lib.pmx_attention_check(C.byref(out), raw_stream(dev)))
 
 
 def _prompt(query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_heads, head_dim, is_causal, num_kv_heads,
             scale, logit_cap, alibi_slopes, prefix_lens):
     name = "prompt_attention"
-    dev = query.device
-    same_device(name, dev if query.is_cuda else torch.device("cuda"), query=query, key=key, value=value,
-                seqstarts=seqstarts, kvstarts=kvstarts, alibi_slopes=alibi_slopes, prefix_lens=prefix_lens)
+    dev = query.get_device()
+    for t in (query, key, value, seqstarts, kvstarts, alibi_slopes, prefix_lens):
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            same_device(name, dev, query=query, key=key, value=value, seqstarts=seqstarts, kvstarts=kvstarts,
+                        alibi_slopes=alibi_slopes, prefix_lens=prefix_lens)
     code = _code(name, query)
     kv_heads = num_kv_heads or num_heads
     scale = _numbers(name, num_heads, kv_heads, head_dim, scale, logit_cap)
@@ -76,30 +83,31 @@ def _prompt(query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_h
         alibi_slopes = alibi_slopes.to(torch.float32).contiguous()
     max_seqlen, max_kvlen = host_int(name, "max_seqlen", max_seqlen), host_int(name, "max_kvlen", max_kvlen)
     Tq, Tk = q.shape[0], k.shape[0]
+    out = q.new_empty((Tq, num_heads, head_dim))
     if Tq == 0 or Tk == 0:
-        return torch.zeros((Tq, num_heads, head_dim), dtype=q.dtype, device=dev)
-    out = torch.empty((Tq, num_heads, head_dim), dtype=q.dtype, device=dev)
+        return out.zero_()
+    q0, q1, _ = q.stride()
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
     with on_device(dev):
-        ws = workspace(lib.pmx_prompt_attention_workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen,
-                                                                max_kvlen, code), dev)
-        check(lib.pmx_prompt_attention(
+        nbytes = _workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen, max_kvlen, code)
+        ws = workspace(nbytes, q.device) if nbytes else None
+        check(lib.pmx_prompt_attention(PROMPT_ATTENTION_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), seqstarts.data_ptr(), kvstarts.data_ptr(),
-            None if prefix_lens is None else prefix_lens.data_ptr(),
-            None if alibi_slopes is None else alibi_slopes.data_ptr(), out.data_ptr(), Tq, Tk, B, num_heads, kv_heads,
-            head_dim, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), max_seqlen,
-            max_kvlen, 1 if is_causal else 0, scale, logit_cap, code, ws.data_ptr(),
-            ws.numel(), stream_of(q)))
+            0 if prefix_lens is None else prefix_lens.data_ptr(), 0 if alibi_slopes is None else alibi_slopes.data_ptr(),
+            out.data_ptr(), ws.data_ptr() if nbytes else 0, Tq, Tk, B, num_heads, kv_heads, head_dim, q0, q1, k0, k1, v0, v1,
+            max_seqlen, max_kvlen, 1 if is_causal else 0, code, nbytes, scale, logit_cap), raw_stream(dev)))
     return out
 
 
 def _tree(query, current_key, current_value, seqstarts, cachestarts, start_pos, tree_mask, max_seqlen, max_kvlen, cache,
           num_heads, head_dim, num_kv_heads, num_layer, layer_idx, cache_layout, scale, logit_cap):
-    from . import cache_strides
     name = "tree_cache_attention"
-    dev = query.device
-    same_device(name, dev if query.is_cuda else torch.device("cuda"), query=query, current_key=current_key,
-                current_value=current_value, cache=cache, seqstarts=seqstarts, cachestarts=cachestarts,
-                start_pos=start_pos, tree_mask=tree_mask)
+    dev = query.get_device()
+    for t in (query, current_key, current_value, cache, seqstarts, cachestarts, start_pos, tree_mask):
+        if dev < 0 or t.get_device() != dev:
+            same_device(name, dev, query=query, current_key=current_key, current_value=current_value, cache=cache,
+                        seqstarts=seqstarts, cachestarts=cachestarts, start_pos=start_pos, tree_mask=tree_mask)
     code = _code(name, query)
     kv_heads = num_kv_heads or num_heads
     scale = _numbers(name, num_heads, kv_heads, head_dim, scale, logit_cap)
@@ -121,18 +129,20 @@ def _tree(query, current_key, current_value, seqstarts, cachestarts, start_pos, 
     cachestarts, start_pos = index(name, "cachestarts", cachestarts, B), index(name, "start_pos", start_pos, B)
     tree_mask = index(name, "tree_mask", tree_mask, Tq)
     max_seqlen, max_kvlen = host_int(name, "max_seqlen", max_seqlen), host_int(name, "max_kvlen", max_kvlen)
-    out = torch.empty((Tq, num_heads, head_dim), dtype=q.dtype, device=dev)
+    out = q.new_empty((Tq, num_heads, head_dim))
     if Tq == 0 or rows == 0:
         return out.zero_()
+    q0, q1, _ = q.stride()
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
     with on_device(dev):
-        ws = workspace(lib.pmx_tree_cache_attention_workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen,
-                                                                    max_kvlen, code), dev)
-        check(lib.pmx_tree_cache_attention(
+        nbytes = _workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen, max_kvlen, code)
+        ws = workspace(nbytes, q.device) if nbytes else None
+        check(lib.pmx_tree_cache_attention(TREE_ATTENTION_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), cache.data_ptr(), seqstarts.data_ptr(), cachestarts.data_ptr(),
-            start_pos.data_ptr(), tree_mask.data_ptr(), out.data_ptr(), Tq, B, num_heads, kv_heads, head_dim,
-            q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), rows, layer_off, row_stride,
-            kv_stride, head_stride, max_seqlen, max_kvlen, scale, logit_cap, code,
-            ws.data_ptr(), ws.numel(), stream_of(q)))
+            start_pos.data_ptr(), tree_mask.data_ptr(), out.data_ptr(), ws.data_ptr() if nbytes else 0, Tq, B, num_heads,
+            kv_heads, head_dim, q0, q1, k0, k1, v0, v1, rows, layer_off, row_stride, kv_stride, head_stride, max_seqlen,
+            max_kvlen, code, nbytes, scale, logit_cap), raw_stream(dev)))
     return out
 
 
@@ -194,7 +204,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     query, key and value may be views with unit inner stride.  float16, bfloat16, float32, head_dim up to 256."""
     args = (query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_heads, head_dim, is_causal, num_kv_heads,
             scale, float(logit_cap), alibi_slopes, prefix_lens)
-    if torch.onnx.is_in_onnx_export() or wants_grad(query, key, value, alibi_slopes):
+    if exporting() or wants_grad(query, key, value, alibi_slopes):
         return PromptAttention.apply(*args)
     return _prompt(*args)
 
@@ -215,6 +225,6 @@ def tree_cache_attention(query: torch.Tensor, current_key: torch.Tensor, current
     prompt_attention()."""
     args = (query, current_key, current_value, seqstarts, cachestarts, start_pos, tree_mask, max_seqlen, max_kvlen, cache,
             num_heads, head_dim, num_kv_heads, num_layer, layer_idx, cache_layout, scale, float(logit_cap))
-    if torch.onnx.is_in_onnx_export() or wants_grad(query, current_key, current_value, cache):
+    if exporting() or wants_grad(query, current_key, current_value, cache):
         return TreeCacheAttention.apply(*args)
     return _tree(*args)

@@ -13,8 +13,8 @@ from typing import Optional, Tuple
 
 import torch
 
-from ..._cabi import lib, check, stream_of, DTYPE_CODE
-from ._common import heads, index, on_device, same_device, wants_grad
+from ..._cabi import lib, check, DTYPE_CODE, ROTARY_ARGS
+from ._common import exporting, heads, index, on_device, raw_stream, same_device, wants_grad
 
 
 @functools.lru_cache(maxsize=64)
@@ -54,58 +54,68 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling_type: st
     return (C.c_double * (r // 2))(*f), factor
 
 
+@functools.lru_cache(maxsize=64)
+def _table(*args):
+    table, factor = rotary_frequencies(*args)
+    return table, C.addressof(table), factor
+
+
 def _launch(name, query, key, q_weight, k_weight, eps, seqstarts, start_pos, position_ids, rotary_dim, theta,
             interleaved, scaling_type, scaling_factor, original_max_position):
+    dev = query.get_device()
+    for t in (query, key, q_weight, k_weight, seqstarts, start_pos, position_ids):
+        if t is not None and (dev < 0 or t.get_device() != dev):
+            same_device(name, dev, query=query, key=key, query_norm_weight=q_weight, key_norm_weight=k_weight,
+                        seqstarts=seqstarts, start_pos=start_pos, position_ids=position_ids)
     if query.dim() != 3:
         raise ValueError(f"{name}: `query` must be [tokens, num_heads, head_dim], not {tuple(query.shape)}")
     T, Hq, D = query.shape
-    dev = query.device
-    same_device(name, dev if query.is_cuda else torch.device("cuda"), query=query, key=key, query_norm_weight=q_weight,
-                key_norm_weight=k_weight, seqstarts=seqstarts, start_pos=start_pos, position_ids=position_ids)
-    code = DTYPE_CODE.get(query.dtype)
+    dtype = query.dtype
+    code = DTYPE_CODE.get(dtype)
     if code is None:
-        raise TypeError(f"{name}: dtype {query.dtype} is not supported (float16, bfloat16, float32)")
-    q, Hkv = heads(name, "query", query, Hq, D, query.dtype), 0
+        raise TypeError(f"{name}: dtype {dtype} is not supported (float16, bfloat16, float32)")
+    q = heads(name, "query", query, Hq, D, dtype)
+    s0, s1, _ = q.stride()
+    k, Hkv, k0, k1 = None, 0, 0, 0
     if key is not None:
         if key.dim() != 3 or key.shape[0] != T:
             raise ValueError(f"{name}: `key` must be [{T}, num_kv_heads, {D}], not {tuple(key.shape)}")
         Hkv = key.shape[1]
-        k = heads(name, "key", key, Hkv, D, query.dtype)
-    weights = [None, None]
-    for n, (label, w) in enumerate((("query_norm_weight", q_weight), ("key_norm_weight", k_weight))):
-        if w is not None:
-            if tuple(w.shape) != (D,) or w.dtype is not query.dtype:
+        k = heads(name, "key", key, Hkv, D, dtype)
+        k0, k1, _ = k.stride()
+    qw = kw = 0
+    if q_weight is not None:
+        for label, w in (("query_norm_weight", q_weight), ("key_norm_weight", k_weight)):
+            if w.shape != (D,) or w.dtype is not dtype:
                 raise ValueError(f"{name}: `{label}` must be [{D}] in the query's dtype")
-            weights[n] = w.contiguous()
-    B = 0
+        q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+        qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
+    B = ss = sp = ids = 0
     if position_ids is not None:
         position_ids = index(name, "position_ids", position_ids, T)
+        ids = position_ids.data_ptr()
     else:
         if seqstarts is None or start_pos is None:
             raise ValueError(f"{name}: positions come from `position_ids` or from `seqstarts` and `start_pos`")
         B = seqstarts.numel() - 1
-        seqstarts = index(name, "seqstarts", seqstarts, max(B, 1) + 1)
-        start_pos = index(name, "start_pos", start_pos, B)
+        seqstarts, start_pos = index(name, "seqstarts", seqstarts, max(B, 1) + 1), index(name, "start_pos", start_pos, B)
+        ss, sp = seqstarts.data_ptr(), start_pos.data_ptr()
     r = rotary_dim or D
     if r > D:
         raise ValueError(f"{name}: rotary_dim {r} is above head_dim {D}")
-    table, factor = rotary_frequencies(r, theta, scaling_type, scaling_factor, original_max_position)
-    qo = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
-    ko = torch.empty((T, Hkv, D), dtype=q.dtype, device=dev) if key is not None else None
+    _, table, factor = _table(r, theta, scaling_type, scaling_factor, original_max_position)
+    qo = q.new_empty((T, Hq, D))
+    ko = None if k is None else k.new_empty((T, Hkv, D))
     if T == 0 or Hq == 0:
         if ko is not None and ko.numel():
             raise ValueError(f"{name}: there are no query heads")
         return qo, ko
-    if ko is not None and Hkv == 0:
-        key = None
-    at = lambda t: None if t is None else t.data_ptr()
+    if Hkv == 0:
+        kw = 0
     with on_device(dev):
-        check(lib.pmx_rotary_embedding(
-            q.data_ptr(), None if key is None else k.data_ptr(), at(weights[0]), None if key is None else at(weights[1]),
-            eps, qo.data_ptr(), None if key is None else ko.data_ptr(), at(seqstarts) if B else None,
-            at(start_pos) if B else None, at(position_ids), T, B, Hq, Hkv, D, q.stride(0), q.stride(1),
-            k.stride(0) if key is not None else 0, k.stride(1) if key is not None else 0, table, r, factor,
-            1 if interleaved else 0, code, stream_of(q)))
+        check(lib.pmx_rotary_embedding(ROTARY_ARGS.pack(
+            q.data_ptr(), k.data_ptr() if Hkv else 0, qw, kw, qo.data_ptr(), ko.data_ptr() if Hkv else 0, ss, sp, ids, table,
+            T, B, Hq, Hkv, D, s0, s1, k0, k1, r, 1 if interleaved else 0, code, eps, factor), raw_stream(dev)))
     return qo, ko
 
 
@@ -174,7 +184,7 @@ def rotary_position_embedding(query: torch.Tensor, key: Optional[torch.Tensor], 
     `scaling_type` as in rotary_frequencies().  float16, bfloat16, float32; one rounding of the result."""
     args = (query, key, seqstarts, start_pos, position_ids, rotary_dim, theta, interleaved, scaling_type,
             scaling_factor, original_max_position)
-    if torch.onnx.is_in_onnx_export() or wants_grad(query, key):
+    if exporting() or wants_grad(query, key):
         out = RotaryPositionEmbedding.apply(*args)
         return (out, None) if key is None else out
     return _launch("rotary_position_embedding", query, key, None, None, 0.0, *args[2:])
@@ -193,6 +203,6 @@ def qk_norm_rotary_embedding(query: torch.Tensor, key: torch.Tensor, query_norm_
         raise ValueError("qk_norm_rotary_embedding: key and both norm weights are needed")
     args = (query, key, query_norm_weight, key_norm_weight, float(eps), seqstarts, start_pos, position_ids, rotary_dim,
             theta, interleaved, scaling_type, scaling_factor, original_max_position)
-    if torch.onnx.is_in_onnx_export() or wants_grad(query, key, query_norm_weight, key_norm_weight):
+    if exporting() or wants_grad(query, key, query_norm_weight, key_norm_weight):
         return QkNormRotaryEmbedding.apply(*args)
     return _launch("qk_norm_rotary_embedding", *args)

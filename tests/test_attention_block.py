@@ -59,60 +59,76 @@ def test_operators_refuse_cpu_tensors(DB):
 
 
 def test_c_abi_refuses_before_it_launches():
+    from ppl.pmx_b200 import _cabi
     from ppl.pmx_b200._cabi import lib
-    one, none = C.c_void_p(16), None
     f = (C.c_double * 128)(*([1.0] * 128))
 
-    def rotary(**kw):
-        a = dict(q=one, k=one, qw=none, kw=none, eps=0.0, qo=one, ko=one, ss=one, sp=one, ids=none, T=4, B=2, Hq=4, Hkv=2,
-                 D=64, s0=256, s1=64, s2=128, s3=64, f=f, r=64, m=1.0, il=0, dt=0, st=none)
-        a.update(kw)
-        return lib.pmx_rotary_embedding(*a.values())
+    def caller(fn, packer, **defaults):
+        def call(**kw):
+            assert set(kw) <= set(defaults)
+            return fn(packer.pack(*{**defaults, **kw}.values()), None)
+        return call
 
-    assert rotary(q=none) == -1 and rotary(qo=none) == -1 and rotary(f=none) == -1
+    rotary = caller(lib.pmx_rotary_embedding, _cabi.ROTARY_ARGS, q=16, k=16, qw=0, kw=0, qo=16, ko=16, ss=16, sp=16, ids=0,
+                    f=C.addressof(f), T=4, B=2, Hq=4, Hkv=2, D=64, s0=256, s1=64, s2=128, s3=64, r=64, il=0, dt=0, eps=0.0,
+                    m=1.0)
+    assert rotary(q=0) == -1 and rotary(qo=0) == -1 and rotary(f=0) == -1
     assert rotary(T=0) == -1 and rotary(Hq=0) == -1 and rotary(D=0) == -1
-    assert rotary(k=none) == -1 and rotary(Hkv=0) == -1 and rotary(ko=none) == -1
-    assert rotary(ss=none) == -1 and rotary(sp=none) == -1 and rotary(B=0) == -1
+    assert rotary(k=0) == -1 and rotary(Hkv=0) == -1 and rotary(ko=0) == -1
+    assert rotary(ss=0) == -1 and rotary(sp=0) == -1 and rotary(B=0) == -1
     assert rotary(r=63) == -1 and rotary(r=66) == -1 and rotary(r=0) == -1 and rotary(r=258, D=512) == -2
-    assert rotary(qw=one) == -1 and rotary(kw=one) == -1 and rotary(dt=7) == -2
+    assert rotary(qw=16) == -1 and rotary(kw=16) == -1 and rotary(dt=7) == -2
 
-    def prompt(**kw):
-        a = dict(q=one, k=one, v=one, ss=one, ks=one, pre=none, sl=none, out=one, Tq=4, Tk=4, B=1, Hq=4, Hkv=2, D=64, q0=256,
-                 q1=64, k0=128, k1=64, v0=128, v1=64, ms=4, mk=4, causal=1, scale=1.0, cap=0.0, dt=0, ws=none, wb=0, st=none)
-        a.update(kw)
-        return lib.pmx_prompt_attention(*a.values())
-
+    prompt = caller(lib.pmx_prompt_attention, _cabi.PROMPT_ATTENTION_ARGS, q=16, k=16, v=16, ss=16, ks=16, pre=0, sl=0, out=16,
+                    ws=0, Tq=4, Tk=4096, B=1, Hq=4, Hkv=2, D=64, q0=256, q1=64, k0=128, k1=64, v0=128, v1=64, ms=4, mk=4096,
+                    causal=1, dt=0, wb=0, scale=1.0, cap=0.0)
     for name in ("q", "k", "v", "ss", "ks", "out"):
-        assert prompt(**{name: none}) == -1
+        assert prompt(**{name: 0}) == -1
     for name in ("Tq", "Tk", "B", "Hq", "Hkv", "D", "ms", "mk"):
         assert prompt(**{name: 0}) == -1, name
-    assert prompt(Hq=3) == -1 and prompt(D=257) == -2 and prompt(dt=5) == -2 and prompt(B=1 << 20) == -2
+    assert prompt(Hq=3) == -1 and prompt(D=257) == -2 and prompt(dt=5) == -2 and prompt(B=1 << 21) == -2
     assert prompt(scale=0.0) == -1 and prompt(scale=float("inf")) == -1 and prompt(scale=float("nan")) == -1
     assert prompt(cap=-1.0) == -1 and prompt(cap=float("inf")) == -1
-    assert prompt() == -4                                     # no workspace
+    assert prompt() == -4 and prompt(ws=16, wb=64) == -4                # few rows, many keys: a split, and so a workspace
+    assert prompt(ws=8, wb=1 << 30) == -3
+    assert lib.pmx_attention_workspace_bytes(4, 1, 4, 2, 64, 4, 100, 0) == 0
+    assert lib.pmx_attention_workspace_bytes(4, 1, 4, 2, 64, 4, 4096, 2) == 0           # 32-bit tensors: the plain kernel
 
-    def tree(**kw):
-        a = dict(q=one, k=one, v=one, cache=one, ss=one, cs=one, sp=one, mask=one, out=one, Tq=4, B=1, Hq=4, Hkv=2, D=64,
-                 q0=256, q1=64, k0=128, k1=64, v0=128, v1=64, rows=9, lo=0, rs=256, kvs=128, hs=64, ms=4, mk=4, scale=1.0,
-                 cap=0.0, dt=0, ws=none, wb=0, st=none)
-        a.update(kw)
-        return lib.pmx_tree_cache_attention(*a.values())
-
+    tree = caller(lib.pmx_tree_cache_attention, _cabi.TREE_ATTENTION_ARGS, q=16, k=16, v=16, cache=16, ss=16, cs=16, sp=16,
+                  mask=16, out=16, ws=0, Tq=4, B=1, Hq=4, Hkv=2, D=64, q0=256, q1=64, k0=128, k1=64, v0=128, v1=64, rows=9, lo=0,
+                  rs=256, kvs=128, hs=64, ms=4, mk=4096, dt=0, wb=0, scale=1.0, cap=0.0)
     for name in ("q", "k", "v", "cache", "ss", "cs", "sp", "mask", "out"):
-        assert tree(**{name: none}) == -1
+        assert tree(**{name: 0}) == -1
     assert tree(ms=65) == -2 and tree(rows=0) == -1 and tree(mk=0) == -1 and tree(Hq=5) == -1 and tree() == -4
 
-    def compact(**kw):
-        a = dict(cache=one, cs=one, sp=one, ast=one, ai=one, B=1, n=4, most=4, layers=1, heads=1, D=64, rows=8, rs=128,
-                 ls=1024, kvs=64, hs=64, dt=0, st=none)
-        a.update(kw)
-        return lib.pmx_compact_cache(*a.values())
-
+    compact = caller(lib.pmx_compact_cache, _cabi.COMPACT_CACHE_ARGS, cache=16, cs=16, sp=16, ast=16, ai=16, B=1, n=4, most=4,
+                     layers=1, heads=1, D=64, rows=8, rs=128, ls=1024, kvs=64, hs=64, dt=0)
     for name in ("cache", "cs", "sp", "ast", "ai"):
-        assert compact(**{name: none}) == -1
+        assert compact(**{name: 0}) == -1
     for name in ("B", "n", "most", "layers", "heads", "D", "rows"):
         assert compact(**{name: 0}) == -1
     assert compact(most=65) == -2 and compact(B=70000) == -2 and compact(dt=3) == -2
+    for fn in (lib.pmx_rotary_embedding, lib.pmx_prompt_attention, lib.pmx_tree_cache_attention, lib.pmx_compact_cache):
+        assert fn(None, None) == -1
+
+
+def test_packed_arguments_match_the_header():
+    """The structs of include/pmx_moe.h, member by member: 8-byte members in the packers' order."""
+    import os
+    import re
+    from ppl.pmx_b200 import _cabi
+    text = open(os.path.join(os.path.dirname(_cabi.PKG), "..", "include", "pmx_moe.h")).read()
+    for name, packer in (("rotary", _cabi.ROTARY_ARGS), ("prompt_attention", _cabi.PROMPT_ATTENTION_ARGS),
+                         ("tree_attention", _cabi.TREE_ATTENTION_ARGS), ("compact_cache", _cabi.COMPACT_CACHE_ARGS)):
+        body = re.search(r"typedef struct pmx_%s_args \{(.*?)\} pmx_%s_args;" % (name, name), text, re.S).group(1)
+        kinds = ""
+        for decl in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";")[:-1]:
+            # pointers, 64-bit integers, doubles
+            assert "*" in decl or "int64_t" in decl or "double" in decl, decl
+            kinds += ("d" if "double" in decl and "*" not in decl else "q") * (decl.count(",") + 1)
+        q, d = kinds.count("q"), kinds.count("d")
+        assert kinds == "q" * q + "d" * d
+        assert packer.format == "=%dq" % q + ("%dd" % d if d else "") and packer.size == 8 * (q + d)
 
 
 def test_export_as_custom_operators(DB):
