@@ -214,7 +214,7 @@ int attention_check(int out[4], cudaStream_t s) {
 
 size_t attention_workspace_bytes(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_seqlen,
                                  int64_t max_kvlen, int dtype) {
-  return tc::tc_workspace(tc::plan_tc(Tq, B, Hq, Hkv, D, max_seqlen, max_kvlen, dtype), Tq, Hq, D);
+  return tc::tc_workspace(tc::plan_tc(Tq, B, Hq, Hkv, D, max_seqlen, max_kvlen, dtype), Tq, B, Hq, Hkv, D);
 }
 
 // what the two operators share once their own arguments are in place
@@ -237,7 +237,7 @@ int run_attention(AttnArgs& a, const P& p, const char* name, cudaStream_t s) {
   if (!(a.scale > 0.f) || a.scale > 3e38f) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", name);
   if (!(a.cap >= 0.f) || a.cap > 3e38f) return fail(PMX_ERR_INVALID_ARGUMENT, "%s: logit_cap must be finite and not negative", name);
   const tc::TcPlan plan = tc::plan_tc(p.tokens, p.sequences, p.num_heads, p.num_kv_heads, p.head_dim, p.max_seqlen, p.max_kvlen, (int)p.dtype);
-  const size_t need = tc::tc_workspace(plan, p.tokens, p.num_heads, p.head_dim);
+  const size_t need = tc::tc_workspace(plan, p.tokens, p.sequences, p.num_heads, p.num_kv_heads, p.head_dim);
   if (need && (!p.workspace || p.workspace_bytes < (int64_t)need))
     return fail(PMX_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %lld given", name, need, (long long)p.workspace_bytes);
   if (need && !aligned16(p.workspace)) return fail(PMX_ERR_ALIGNMENT, "%s: the workspace must be 16-byte aligned", name);

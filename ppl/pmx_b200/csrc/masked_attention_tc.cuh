@@ -1,31 +1,40 @@
 // The tensor-core kernel of masked_attention.cu (included there, inside its namespaces): 16-bit tensors, head
 // sizes up to 128.
 //
-// A CTA computes one or two tiles of 128 rows against the keys of their sequence, 128 at a time.  A row is a
+// A work item is one or two tiles of 128 rows against (a run of) the keys of their sequence, 128 at a time.  A row is a
 // (query token, query head) of ONE key head: the G query heads that share it are packed into the tile
-// (128 / G tokens of them), so each key and value crosses to the SM once for the whole group.
-//   warp 8   TMA: keys and values through a ring of 128-row buffers (128-byte swizzle)
+// (128 / G tokens of them), so each key and value crosses to the SM once for the whole group.  One CTA per SM
+// walks its items; its warps each run through all of them, so that the loads and products of the next item
+// begin under the last one's end:
+//   warp 8   makes the items (a queue in shared memory) and issues the TMA loads: keys and values through a ring
+//            of 128-row buffers (128-byte swizzle)
 //   warp 9   one thread issues the tcgen05 products: S_w = Q_w K^T into tensor memory columns [128 w, +128),
 //            O_w += P_w V into columns [256 + 128 w, +128); P_w is read from tensor memory, V is the MN-major operand
 //   warps 0-3 and 4-7  the softmax of S_0 and S_1, one thread per row (a thread owns a tensor memory lane, so the
 //            row's maximum and sum need no exchange); P_w overwrites S_w in 16 bits
-//   warps 10, 11  go over those value tiles of which some rows see a part only
-// With more than 128 rows (PAIR) the two tiles share the keys; with fewer, both softmax halves work on the same
-// rows, on the even and the odd key tiles, and meet at the end: either way one half's softmax runs
-// beside the other's products.  The running maximum moves only when a row's new maximum lies more than 2^8
-// above it, so that O in tensor memory is rescaled rarely; probabilities stay below 2^8, exact in the 16-bit types'
-// range, and the sum divides the same scale out again.
-// Few rows and many keys: the key tiles are dealt out over several CTAs, whose partial results (fp32, with maximum
-// and sum) a second kernel merges.
+//   warps 10, 11  go over those value tiles of which some rows see a part only, and store drafted keys and values
+// With more than 128 rows (`pair`) the two tiles share the keys; an item is one block of rows, the longest first.  With
+// fewer, both softmax halves work on the same rows, on the even and the odd key tiles, and meet at the end; the
+// key tiles of all (sequence, key head) pairs are then dealt out evenly over the CTAs as one long list, and what a cut
+// leaves in pieces is merged by a second kernel (fp32 results with maximum and sum).  Pairs with so few CTAs that SMs
+// would idle split their keys too.
+//
+// The bound is the tensor pipe and, next to it, the exponentials: per 128 x 128 scores 1024 cycles of products (head
+// size 128) against 1024 of the special function unit, and a tile's softmax lies between its own two products.  So a
+// half's softmax runs beside the other half's products, and is kept short.  The running maximum moves only when a
+// row's new maximum lies more than 2^8 above it, so that O in tensor memory is rescaled rarely; probabilities stay below
+// 2^8, exact in the 16-bit types' range, and the sum divides the same scale out again.
 //
 // A masked score becomes -inf whatever the product holds.  A masked VALUE needs more: 0 * inf and 0 * NaN are NaN in
 // the second product, so in the tiles that are not seen whole by every row, values that are not finite are replaced by
-// zeros in shared memory, and if there were any among the sequence's own, the epilogue adds them back for the rows
-// that see them.
+// zeros in shared memory, and if there were any among the sequence's own, the end of the item adds them back for the
+// rows that see them.
 constexpr int kTile = 128;                  // keys of a tile, rows of a tile
 constexpr int kRing = 5;                    // ring buffers: two keys and two values in use, one on the way
 constexpr int kAttnThreads = 384;
 constexpr int kMaxSplits = 32;
+constexpr int kQueue = 4;                   // items under way
+constexpr int kMinTiles = 4;                // key tiles that a CTA should have before work is cut finer
 constexpr float kLazy = 8.0f;               // log2 of how far a maximum may run ahead
 constexpr unsigned long long kAttnWaitNs = 2000000000ull;
 
@@ -37,18 +46,38 @@ struct TileMaps {
 
 struct TcArgs {
   AttnArgs a;
-  float* part_o;                            // [splits][Tq * Hq][D]
-  float2* part_ml;                          // [splits][Tq * Hq] maximum (log2), sum
+  // pair: partial results [splits][Tq * Hq][D], maximum (log2) and sum [splits][Tq * Hq].  Otherwise [2 * CTAs][128][D] and
+  // [2 * CTAs][128]: a CTA's first piece in slot 2c when it begins inside an item, its last in 2c + 1 when it ends inside;
+  // pieces[b * Hkv + h] = the CTAs (first, last) that share the item.
+  float* part_o;
+  float2* part_ml;
+  int2* pieces;
   int group, tokens;                        // query heads per key head, tokens of a row tile
-  int row_blocks, splits, pair, zero_ctas;
+  int row_blocks, splits, pair;
+  int flat;                                 // not pair: cut the list of key tiles evenly (otherwise whole items)
+};
+
+struct Work {
+  int b, h, slot;      // slot: of the partial result, -1: none; h < 0: the end
+  Sequence s;
+  int tok0;            // first token of the item's rows, in the sequence
+  int halves;          // row tiles in use (1 without pair)
+  int t0, nt[2];       // first key tile; tiles of each row tile (without pair: nt[0] is the item's)
+  int drafted;         // index of the drafted tokens' tile, -1: none
+  int partial;         // first tile that some row does not see whole
+  int stores;          // this item stores the sequence's drafted keys and values of this head
+  int number;          // of the item in this CTA, from 1
 };
 
 struct Ctl {
   uint64_t full[kRing], empty[kRing], raw[kRing];
-  uint64_t q_full, s_full[2], p_ready[2], o_full[2];
+  uint64_t q_full, q_empty, s_full[2], p_ready[2][2], o_full[2];
+  uint64_t work_full[kQueue], work_empty[kQueue];
+  float2 ml[256];
+  Work work[kQueue];
+  volatile int bad[kQueue];                 // number of the last item in this queue place that had a bad value
   uint32_t tmem;
   volatile int abort;
-  int any_bad;
 };
 
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* c, int role, int tile) {
@@ -77,16 +106,28 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem desc]
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
 }
+// D[tmem] = A * B ("first") or D += A * B ("more"), A from shared memory (descriptor) or from tensor memory ("ts")
+#define PMX_UMMA(name, a_type, a_con, a_brackets_l, a_brackets_r, accumulate)                                        \
+  __device__ __forceinline__ void name(uint32_t d_tmem, a_type a, uint64_t b_desc, uint32_t idesc) {                   \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, " accumulate                                                   \
+                 ", 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], " a_brackets_l "%1" a_brackets_r ", %2, %3, p;\n\t}" \
+                 ::"r"(d_tmem), a_con(a), "l"(b_desc), "r"(idesc)                                                      \
+                 : "memory");                                                                                          \
+  }
+PMX_UMMA(umma_f16_first, uint64_t, "l", "", "", "0")
+PMX_UMMA(umma_f16_more, uint64_t, "l", "", "", "1")
+PMX_UMMA(umma_f16_ts_first, uint32_t, "r", "[", "]", "0")
+PMX_UMMA(umma_f16_ts_more, uint32_t, "r", "[", "]", "1")
+#undef PMX_UMMA
 // Shared-memory descriptor of an MN-major operand: rows (K) of 64 values = 128 bytes with the 128-byte swizzle, 8-row
 // groups 1024 bytes apart; the next 64 values of MN are a 128-row block further.
 __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
@@ -122,10 +163,70 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// waits for the loads from tensor memory before; the registers of the last one pass through, so that no use of
+// them can move in front
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// ---- two 32-bit values per instruction
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair2(f32x2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {     // NaN wins
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 __device__ __forceinline__ float rcp(float x) {
   float y;
@@ -166,56 +267,123 @@ __device__ __forceinline__ uint32_t not_finite2(uint32_t w) {
   return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
 }
 
-// the share of the key tiles that one CTA takes, and what its rows see
-struct Work {
-  int b, h, x, split;
-  Sequence s;
-  int tok0;            // first token of the CTA's rows, in the sequence
-  int halves;          // row tiles in use (1 without PAIR)
-  int t0, nt[2];       // first key tile; tiles of each row tile (without PAIR: nt[0] is the CTA's)
-  int drafted;         // index of the drafted tokens' tile, -1: none
-  int partial;         // first tile that some row does not see whole
-};
-
-__device__ __forceinline__ Work make_work(const TcArgs& p, int idx) {
-  Work w;
+// Key tiles that rows [tok0, tok0 + tokens) of the sequence need, the drafted tokens' tile included.
+__device__ __forceinline__ int key_tiles(const AttnArgs& a, const Sequence& s, int tok0, int tokens) {
+  const int last = tok0 + tokens - 1;
+  const int64_t seen = visible(a, s, last < s.n ? last : s.n - 1);
+  return (int)((seen + kTile - 1) / kTile) + (a.tree_mask ? 1 : 0);
+}
+// What is left of a Work once b, h, s and tok0 are known: the tiles of its rows, cut to [t0, t1).
+__device__ __forceinline__ void finish_work(const TcArgs& p, Work& w, int t0, int t1) {
   const AttnArgs& a = p.a;
-  // row blocks that see the most keys first
-  const int per = a.B * a.Hkv * p.splits;
-  w.x = p.row_blocks - 1 - idx / per;
-  idx %= per;
-  w.split = idx % p.splits;
-  idx /= p.splits;
-  w.h = idx % a.Hkv;
-  w.b = idx / a.Hkv;
-  w.s = load_sequence(a, w.b);
-  const int block_tokens = p.pair ? 2 * p.tokens : p.tokens;
-  w.tok0 = w.x * block_tokens;
-  w.halves = 0;
-  w.drafted = -1;
-  w.t0 = w.nt[0] = w.nt[1] = w.partial = 0;
-  if (w.tok0 >= w.s.n) return w;
   w.halves = p.pair && w.tok0 + p.tokens < w.s.n ? 2 : 1;
-  int total[2];
-  const int64_t first = visible(a, w.s, w.tok0);
-  w.partial = (int)(first / kTile);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int last = w.tok0 + (i + 1) * p.tokens - 1;
-    const int64_t seen = visible(a, w.s, last < w.s.n ? last : w.s.n - 1);
-    total[i] = (int)((seen + kTile - 1) / kTile);
-    if (a.tree_mask) w.drafted = total[i]++;
-  }
-  if (w.halves == 1) total[1] = total[0];
-  // contiguous shares of the longer row tile's key tiles
-  const int share = (total[1] + p.splits - 1) / p.splits;
-  w.t0 = w.split * share < total[1] ? w.split * share : total[1];
-  const int t1 = w.t0 + share < total[1] ? w.t0 + share : total[1];
-  w.nt[0] = (total[0] < t1 ? total[0] : t1) - w.t0;
+  w.partial = (int)(visible(a, w.s, w.tok0) / kTile);
+  const int n0 = key_tiles(a, w.s, w.tok0, p.tokens);
+  const int n1 = w.halves == 2 ? key_tiles(a, w.s, w.tok0, 2 * p.tokens) : n0;
+  w.drafted = a.tree_mask ? n1 - 1 : -1;
+  if (t1 > n1) t1 = n1;
+  w.t0 = t0 < t1 ? t0 : t1;
+  w.nt[0] = (n0 < t1 ? n0 : t1) - w.t0;
   if (w.nt[0] < 0) w.nt[0] = 0;
   w.nt[1] = w.halves == 2 ? t1 - w.t0 : 0;
-  return w;
+  w.stores = a.tree_mask && w.tok0 == 0 && t0 == 0;
 }
+
+// The items of one CTA, in order.  Run by all lanes of a warp.
+struct Items {
+  int at, step, count;            // pair, or whole items: of the list of all items
+  int b;                          // flat: the sequence that [base, base + Hkv * tiles) of the list of key tiles belongs to
+  int64_t base, u, u1, total;
+  int tiles, ctas;
+  Sequence s;
+  __device__ __forceinline__ int tiles_of(const TcArgs& p, int seq, Sequence& q) {
+    q = load_sequence(p.a, seq);
+    if (q.n == 0) return 0;
+    const int t = key_tiles(p.a, q, 0, p.tokens);
+    return t < 1 ? 1 : t;         // rows that see nothing still have a result
+  }
+  __device__ __forceinline__ void start(const TcArgs& p) {
+    const AttnArgs& a = p.a;
+    if (!p.flat) {
+      at = (int)blockIdx.x;
+      step = (int)gridDim.x;
+      count = p.row_blocks * a.B * a.Hkv * p.splits;
+      return;
+    }
+    const int lane = threadIdx.x & 31;
+    int64_t sum = 0;
+    Sequence q;
+    for (int i = lane; i < a.B; i += 32) sum += tiles_of(p, i, q);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    total = sum * a.Hkv;
+    const int64_t most = total / kMinTiles;
+    ctas = (int)(most < 1 ? 1 : (most < (int64_t)gridDim.x ? most : (int64_t)gridDim.x));
+    u = (int)blockIdx.x < ctas ? (int64_t)blockIdx.x * total / ctas : total;
+    u1 = (int)blockIdx.x < ctas ? (int64_t)(blockIdx.x + 1) * total / ctas : total;
+    if (u >= u1) return;
+    // the sequence that u falls into
+    base = 0;
+    for (int i0 = 0; i0 < a.B; i0 += 32) {
+      const int i = i0 + lane;
+      int64_t end = i < a.B ? (int64_t)tiles_of(p, i, q) * a.Hkv : 0;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, end, o);
+        if (lane >= o) end += v;
+      }
+      const unsigned past = __ballot_sync(0xFFFFFFFFu, base + end > u);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b = i0 + l;
+        if (l) base += __shfl_sync(0xFFFFFFFFu, end, l - 1);
+        break;
+      }
+      base += __shfl_sync(0xFFFFFFFFu, end, 31);
+    }
+    tiles = tiles_of(p, b, s);
+  }
+  __device__ __forceinline__ bool next(const TcArgs& p, Work& w) {
+    const AttnArgs& a = p.a;
+    if (!p.flat) {
+      for (; at < count; at += step) {
+        // row blocks that see the most keys first
+        const int per = a.B * a.Hkv * p.splits;
+        int idx = at % per;
+        w.slot = p.splits > 1 ? idx % p.splits : -1;
+        const int split = idx % p.splits;
+        idx /= p.splits;
+        w.h = idx % a.Hkv;
+        w.b = idx / a.Hkv;
+        w.tok0 = (p.row_blocks - 1 - at / per) * (p.pair ? 2 : 1) * p.tokens;
+        w.s = load_sequence(a, w.b);
+        if (w.tok0 >= w.s.n) continue;
+        const int all = key_tiles(a, w.s, w.tok0, (p.pair ? 2 : 1) * p.tokens);
+        const int share = (all + p.splits - 1) / p.splits;
+        finish_work(p, w, split * share, (split + 1) * share);
+        at += step;
+        return true;
+      }
+      return false;
+    }
+    if (u >= u1) return false;
+    while (u >= base + (int64_t)tiles * a.Hkv) {
+      base += (int64_t)tiles * a.Hkv;
+      tiles = tiles_of(p, ++b, s);
+    }
+    const int64_t in = u - base;
+    const int t0 = (int)(in % tiles), left = tiles - t0, take = u1 - u < left ? (int)(u1 - u) : left;
+    w.b = b;
+    w.h = (int)(in / tiles);
+    w.s = s;
+    w.tok0 = 0;
+    finish_work(p, w, t0, t0 + take);
+    w.slot = t0 > 0 ? 2 * (int)blockIdx.x : (take < tiles ? 2 * (int)blockIdx.x + 1 : -1);
+    if (t0 == 0 && (threadIdx.x & 31) == 0)       // the CTA that holds the first tile says who shares the item
+      p.pieces[(int64_t)b * a.Hkv + w.h] =
+          make_int2((int)blockIdx.x, (int)(((u + tiles) * ctas - 1) / total));
+    u += take;
+    return true;
+  }
+};
 
 // rows of a key tile that hold keys of the sequence
 __device__ __forceinline__ int tile_rows(const Work& w, int t) {
@@ -224,71 +392,43 @@ __device__ __forceinline__ int tile_rows(const Work& w, int t) {
   return (int)(left < kTile ? left : kTile);
 }
 
+// Adds to 8 columns of a row's result the values that are not finite, of the keys the row sees in the tiles that were
+// cleaned.  Rare, and kept out of the way of the registers of those who call it.
+struct Cols8 { float v[8]; };
+template <typename T>
+__device__ __noinline__ Cols8 add_bad(Cols8 x, const AttnArgs* ap, const Work* wp, int col, int64_t limit, uint64_t bits,
+                                      int total) {
+  const AttnArgs& a = *ap;
+  const Work& w = *wp;
+  for (int i = w.partial > w.t0 ? w.partial - w.t0 : 0; i < total; ++i) {
+    const int t = w.t0 + i;
+    const bool draft = t == w.drafted;
+    const int rows = tile_rows(w, t);
+    for (int j = 0; j < rows; ++j) {
+      if (!(draft ? (bits >> j & 1) : (int64_t)t * kTile + j < limit)) continue;
+      const T* src = draft ? reinterpret_cast<const T*>(a.cur.v) + (w.s.q0 + j) * a.cur.v_row + w.h * a.cur.v_head
+                           : reinterpret_cast<const T*>(a.past.v) + (w.s.kv0 + (int64_t)t * kTile + j) * a.past.v_row + w.h * a.past.v_head;
+      float f[8];
+      unpack16<T>(ld_stream16(src + col), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (!isfinite(f[e])) x.v[e] += f[e];
+    }
+  }
+  return x;
+}
+
 template <typename T, int DP, bool SCORE>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TcArgs p) {
   constexpr int kTileBytes = kTile * DP * 2;
   constexpr int kBlockBytes = kTile * 128;          // 64 columns of a tile
   constexpr int kDBlocks = DP / 64;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + (2 + kRing) * kTileBytes);
   const AttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
-  pdl_wait();
-  const int work_ctas = p.row_blocks * a.B * a.Hkv * p.splits;
-  if ((int)blockIdx.x >= work_ctas) {
-    // rows of no sequence: zeros, or partial results that count for nothing
-    const int64_t lo = clamp64(__ldcg(a.seqstarts), 0, a.Tq), hi = clamp64(__ldcg(a.seqstarts + a.B), lo, a.Tq);
-    const int64_t rows = (lo + a.Tq - hi) * a.Hq, step = (int64_t)p.zero_ctas * (kAttnThreads / 32);
-    for (int64_t r = ((int64_t)blockIdx.x - work_ctas) * (kAttnThreads / 32) + warp; r < rows; r += step) {
-      const int64_t row = r < lo * a.Hq ? r : r + (hi - lo) * a.Hq;
-      if (p.splits == 1) {
-        T* out = reinterpret_cast<T*>(a.out) + row * a.D;
-        for (int d = lane; d < a.D; d += 32) out[d] = Elem<T>::from_f(0.f);
-      } else if (lane < p.splits) {
-        p.part_ml[(int64_t)lane * a.Tq * a.Hq + row] = make_float2(-INFINITY, 0.f);
-      }
-    }
-    return;
-  }
-  const Work w = make_work(p, (int)blockIdx.x);
-  if (w.halves == 0) return;
-  // without PAIR the two softmax halves take turns on the CTA's tiles
-  const int total = p.pair ? (w.nt[1] > w.nt[0] ? w.nt[1] : w.nt[0]) : w.nt[0];
-  const int rows_tile = p.tokens * p.group;
-  // the row of a softmax thread
-  const int half = warp >> 2, r = threadIdx.x & 127;
-  const int tok = w.tok0 + (p.pair ? half * p.tokens : 0) + r / p.group;
-  const bool row_ok = warp < 8 && r < rows_tile && tok < w.s.n;
-  const int head = w.h * p.group + r % p.group;
-  const int64_t out_row = (w.s.q0 + tok) * a.Hq + head;
-  if (a.tree_mask && w.x == 0 && w.split == 0) {
-    // the sequence's new keys and values go into the cache, where this launch does not read them
-    for (int i = threadIdx.x; i < w.s.n * (a.D / 8) * 2; i += kAttnThreads) {
-      const int ch = i % (a.D / 8), kv = i / (a.D / 8) & 1, t = i / (a.D / 8) >> 1;
-      const int64_t row = w.s.kv0 + w.s.len + t;
-      if (row >= a.past.rows) continue;
-      const T* src = kv ? reinterpret_cast<const T*>(a.cur.v) + (w.s.q0 + t) * a.cur.v_row + w.h * a.cur.v_head
-                        : reinterpret_cast<const T*>(a.cur.k) + (w.s.q0 + t) * a.cur.k_row + w.h * a.cur.k_head;
-      T* dst = kv ? reinterpret_cast<T*>(const_cast<void*>(a.past.v)) + row * a.past.v_row + w.h * a.past.v_head
-                  : reinterpret_cast<T*>(const_cast<void*>(a.past.k)) + row * a.past.k_row + w.h * a.past.k_head;
-      *reinterpret_cast<uint4*>(dst + ch * 8) = ld_stream16(src + ch * 8);
-    }
-  }
-  if (total == 0) {
-    if (row_ok && (p.pair || half == 0)) {
-      if (p.splits == 1) {
-        T* out = reinterpret_cast<T*>(a.out) + out_row * a.D;
-        for (int d = 0; d < a.D; d += 8) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
-      } else {
-        p.part_ml[(int64_t)w.split * a.Tq * a.Hq + out_row] = make_float2(-INFINITY, 0.f);
-      }
-    }
-    return;
-  }
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&ctl->full[i], 1);
@@ -296,14 +436,26 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
       mbar_init(&ctl->raw[i], 1);
     }
     mbar_init(&ctl->q_full, 1);
+    mbar_init(&ctl->q_empty, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->s_full[i], 1);
-      mbar_init(&ctl->p_ready[i], 4);
+      mbar_init(&ctl->p_ready[i][0], 4);
+      mbar_init(&ctl->p_ready[i][1], 4);
       mbar_init(&ctl->o_full[i], 1);
     }
-    ctl->abort = 0;
-    ctl->any_bad = 0;
+    for (int i = 0; i < kQueue; ++i) {
+      mbar_init(&ctl->work_full[i], 1);
+      mbar_init(&ctl->work_empty[i], 11);             // 8 softmax warps, the products' thread, 2 cleaning warps
+      ctl->bad[i] = 0;
+    }
+    // the swizzled tiles need 1024-byte boundaries: the dynamic shared memory of a kernel without static shared
+    // memory begins on one; should it ever not, the kernel says so instead of computing nonsense
+    ctl->abort = (smem_u32(smem) & 1023u) != 0;
+    if (ctl->abort && atomicExch(&g_attention_status[0], 1) != 1) g_attention_status[1] = 99;
     fence_barrier_init();
+    prefetch_tensormap(&maps.q);
+    prefetch_tensormap(&maps.k);
+    prefetch_tensormap(&maps.v);
   }
   if (warp == 9) {
     tmem_alloc(&ctl->tmem, 512);
@@ -312,389 +464,578 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl->tmem;
+  pdl_wait();
+  // All 512 columns are this block's, so they begin at column 0 and addresses are constants; checked all the same.
+  constexpr uint32_t tmem = 0;
+  if (ctl->tmem != 0 && threadIdx.x == 0) {
+    ctl->abort = 1;
+    if (atomicExch(&g_attention_status[0], 1) != 1) g_attention_status[1] = 98;
+  }
   const uint32_t q_addr = smem_u32(smem), ring = q_addr + 2 * kTileBytes;
-  // Order of the ring: the keys of the first `lag` tiles, then values and keys in turn.  Entry of the values of tile i:
+  const int rows_tile = p.tokens * p.group;
+  // Order of the ring within an item: the keys of the first `lag` tiles, then values and keys in turn.
   const int lag = p.pair ? 1 : 2;
-  auto v_entry = [&](int i) { return 2 * i + lag < total + i ? 2 * i + lag : total + i; };
+  auto tiles_of = [&](const Work& w) { return w.nt[0] > w.nt[1] ? w.nt[0] : w.nt[1]; };
 
-  // The softmax warpgroups hold a row of scores in registers; the third one needs few.  216 x 256 + 56 x 128 =
-  // 62464 of the 168 x 384 = 64512 registers that the block starts with.
+  // The softmax warpgroups hold a row of scores in registers; the third one needs few.  208 x 256 + 80 x 128 =
+  // 63488 of the 168 x 384 = 64512 registers that the block starts with.
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == 8) {
-    // ------------------------------------------------------------------ TMA
-    if (lane == 0) {
-      prefetch_tensormap(&maps.k);
-      prefetch_tensormap(&maps.v);
-      mbar_expect_tx(&ctl->q_full, (uint32_t)(w.halves * kDBlocks * 128 * rows_tile));
-      for (int i = 0; i < w.halves; ++i)
-        for (int d = 0; d < kDBlocks; ++d)
-          tma_load_3d(q_addr + i * kTileBytes + d * kBlockBytes, &maps.q, &ctl->q_full, d * 64, w.h * p.group,
-                      (int)w.s.q0 + w.tok0 + i * p.tokens);
-      int slot = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      auto load = [&](int i, bool values) {
-        ok = wait_bar(&ctl->empty[slot], phase ^ 1u, ctl, 0, i);
-        if (!ok) return;
-        const int t = w.t0 + i;
-        const bool draft = t == w.drafted;
-        uint64_t* bar = values && t >= w.partial ? &ctl->raw[slot] : &ctl->full[slot];
-        const CUtensorMap* map = draft ? (values ? &maps.cv : &maps.ck) : (values ? &maps.v : &maps.k);
-        const int row = draft ? (int)w.s.q0 : (int)w.s.kv0 + t * kTile;
-        mbar_expect_tx(bar, (uint32_t)(kDBlocks * 128 * (draft ? kTreeLimit : kTile)));
-        for (int d = 0; d < kDBlocks; ++d)
-          tma_load_3d(ring + slot * kTileBytes + d * kBlockBytes, map, bar, d * 64, w.h, row);
-        if (++slot == kRing) { slot = 0; phase ^= 1u; }
-      };
-      for (int i = 0; i < lag && i < total && ok; ++i) load(i, false);
-      for (int i = 0; i < total && ok; ++i) {
-        load(i, true);
-        if (ok && i + lag < total) load(i + lag, false);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8) {
+      // ---------------------------------------------------------------- items and loads
+      Items items;
+      items.start(p);
+      int slot = 0, place = 0, number = 0;
+      uint32_t phase = 0, place_phase = 0, q_phase = 0;
+      bool ok = !ctl->abort;
+      while (ok) {
+        Work w;
+        const bool more = items.next(p, w);
+        ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->work_empty[place], place_phase ^ 1u, ctl, 7, number));
+        if (!ok) break;
+        w.number = ++number;
+        if (!more) w.h = -1;
+        if (lane == 0) {
+          ctl->work[place] = w;
+          mbar_arrive(&ctl->work_full[place]);
+        }
+        if (++place == kQueue) { place = 0; place_phase ^= 1u; }
+        if (!more) break;
+        const int total = tiles_of(w);
+        if (total == 0) continue;
+        if (lane == 0) {
+          ok = wait_bar(&ctl->q_empty, q_phase ^ 1u, ctl, 8, number);
+          q_phase ^= 1u;
+          if (ok) {
+            mbar_expect_tx(&ctl->q_full, (uint32_t)(w.halves * kDBlocks * 128 * rows_tile));
+            for (int i = 0; i < w.halves; ++i)
+              for (int d = 0; d < kDBlocks; ++d)
+                tma_load_3d(q_addr + i * kTileBytes + d * kBlockBytes, &maps.q, &ctl->q_full, d * 64, w.h * p.group,
+                            (int)w.s.q0 + w.tok0 + i * p.tokens);
+          }
+          auto load = [&](int i, bool values) {
+            ok = wait_bar(&ctl->empty[slot], phase ^ 1u, ctl, 0, i);
+            if (!ok) return;
+            const int t = w.t0 + i;
+            const bool draft = t == w.drafted;
+            uint64_t* bar = values && t >= w.partial ? &ctl->raw[slot] : &ctl->full[slot];
+            const CUtensorMap* map = draft ? (values ? &maps.cv : &maps.ck) : (values ? &maps.v : &maps.k);
+            const int row = draft ? (int)w.s.q0 : (int)w.s.kv0 + t * kTile;
+            mbar_expect_tx(bar, (uint32_t)(kDBlocks * 128 * (draft ? kTreeLimit : kTile)));
+            for (int d = 0; d < kDBlocks; ++d)
+              tma_load_3d(ring + slot * kTileBytes + d * kBlockBytes, map, bar, d * 64, w.h, row);
+            if (++slot == kRing) { slot = 0; phase ^= 1u; }
+          };
+          for (int i = 0; i < lag && i < total && ok; ++i) load(i, false);
+          for (int i = 0; i < total && ok; ++i) {
+            load(i, true);
+            if (ok && i + lag < total) load(i + lag, false);
+          }
+        }
+        ok = __shfl_sync(0xFFFFFFFFu, (int)ok, 0) != 0;
       }
       if (!ok) {      // leave the copies in flight the time to land
         const unsigned long long t0 = global_ns();
         while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
       }
-    }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------ products
-    if (lane == 0) {
+    } else if (warp == 9) {
+      // ---------------------------------------------------------------- products
+      // The whole warp runs the loop and one elected lane issues: operands that are the same in all lanes stay in
+      // uniform registers.  (One thread on its own needed 125 cycles per product, more than the product takes.)
       const uint32_t idesc_s = make_idesc<T>(128, 128), idesc_d = make_idesc<T>(128, kTreeLimit);
       const uint32_t idesc_o = make_idesc<T>(128, DP) | (1u << 16);      // B is MN-major
-      int slot = 0;
-      uint32_t phase = 0, p_phase[2] = {0, 0};
-      bool ok = wait_bar(&ctl->q_full, 0, ctl, 1, 0);
+      const uint64_t q_desc = smem_desc_sw128(q_addr), k_desc = smem_desc_sw128(ring), v_desc = smem_desc_mn(ring);
+      constexpr uint64_t kTile16 = kTileBytes / 16, kBlock16 = kBlockBytes / 16;
+      int slot = 0, place = 0;
+      uint32_t phase = 0, place_phase = 0, q_phase = 0, p_phase0 = 0, p_phase1 = 0;
+      bool ok = true;
       auto next = [&]() { if (++slot == kRing) { slot = 0; phase ^= 1u; } };
-      auto scores = [&](int q, int i) {             // row tile q and half: S = Q K_i^T from the current slot
-        const uint32_t ka = ring + slot * kTileBytes, qa = q_addr + (p.pair ? q : 0) * kTileBytes;
+      for (;;) {
+        ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->work_full[place], place_phase, ctl, 9, 0));
+        if (!ok) break;
+        const Work& w = ctl->work[place];
+        if (w.h < 0) break;
+        const int n0 = __shfl_sync(0xFFFFFFFFu, w.nt[0], 0), n1 = __shfl_sync(0xFFFFFFFFu, w.nt[1], 0);
+        const int total = n0 > n1 ? n0 : n1;
+        const int drafted = __shfl_sync(0xFFFFFFFFu, w.drafted - w.t0, 0);          // from the item's first tile
+        const int last_rows = __shfl_sync(0xFFFFFFFFu, total > 0 ? tile_rows(w, w.t0 + total - 1) : 0, 0);
+        // the past's last tile may be short too where a drafted tile follows
+        const int prev_rows = __shfl_sync(0xFFFFFFFFu, total > 1 ? tile_rows(w, w.t0 + total - 2) : 0, 0);
+        auto wait = [&](uint64_t* bar, uint32_t parity, int role, int i) {
+          ok = __all_sync(0xFFFFFFFFu, wait_bar(bar, parity, ctl, role, i));
+          tc_fence_after();
+        };
+        // S_q = Q_q K_i^T from the current slot
+        auto scores = [&](int q, int i) {
+          if (elect_one()) {
+            const uint64_t kd = k_desc + slot * kTile16, qd = q_desc + (p.pair ? q : 0) * kTile16;
+            const uint32_t idesc = i == drafted ? idesc_d : idesc_s;
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint32_t off = (kk / 4) * kBlockBytes + (kk % 4) * 32;
-          umma_f16(tmem + q * 128, smem_desc_sw128(qa + off), smem_desc_sw128(ka + off),
-                   w.t0 + i == w.drafted ? idesc_d : idesc_s, kk > 0 ? 1u : 0u);
-        }
-        umma_commit(&ctl->s_full[q]);
-      };
-      auto output = [&](int q, int i, bool first) { // O += P V_i from the current slot
-        const uint32_t va = ring + slot * kTileBytes;
-        const int steps = (tile_rows(w, w.t0 + i) + 15) / 16;
-        for (int kk = 0; kk < steps; ++kk)
-          umma_f16_ts(tmem + 256 + q * 128, tmem + q * 128 + kk * 8, smem_desc_mn(va + kk * 2048), idesc_o,
-                      !first || kk > 0 ? 1u : 0u);
-      };
-      auto wait_p = [&](int q, int i) {
-        ok = wait_bar(&ctl->p_ready[q], p_phase[q], ctl, 3, i);
-        p_phase[q] ^= 1u;
-        tc_fence_after();
-      };
-      auto wait_full = [&](int i) {
-        ok = wait_bar(&ctl->full[slot], phase, ctl, 2, i);
-        tc_fence_after();
-      };
-      if (!p.pair) {
-        for (int i = 0; i < 2 && i < total && ok; ++i) {
-          wait_full(i);
-          if (!ok) break;
-          scores(i, i);
-          umma_commit(&ctl->empty[slot]);
-          next();
-        }
-        for (int i = 0; i < total && ok; ++i) {
-          const int q = i & 1;
-          wait_full(i);
-          if (ok) wait_p(q, i);
-          if (!ok) break;
-          output(q, i, i < 2);
-          umma_commit(&ctl->empty[slot]);
-          next();
-          if (i + 2 < total) {
-            wait_full(i + 2);
-            if (!ok) break;
-            scores(q, i + 2);
-            umma_commit(&ctl->empty[slot]);
-            next();
-          } else {
-            umma_commit(&ctl->o_full[q]);
-          }
-        }
-      } else {
-        if (ok) wait_full(0);
-        if (ok) {
-          for (int q = 0; q < 2; ++q)
-            if (w.nt[q] > 0) scores(q, 0);
-          umma_commit(&ctl->empty[slot]);
-          next();
-        }
-        for (int i = 0; i < total && ok; ++i) {
-          // the current slot holds V_i, the one behind it K_i+1
-          wait_full(i);
-          if (!ok) break;
-          const int v_slot = slot;
-          const uint32_t v_phase = phase;
-          next();
-          const int k_slot = slot;
-          const uint32_t k_phase = phase;
-          for (int q = 0; q < 2 && ok; ++q) {
-            if (i >= w.nt[q]) continue;
-            wait_p(q, i);
-            if (!ok) break;
-            slot = v_slot; phase = v_phase;
-            output(q, i, i == 0);
-            slot = k_slot; phase = k_phase;
-            if (i + 1 < w.nt[q]) {
-              wait_full(i + 1);
-              if (!ok) break;
-              scores(q, i + 1);
-            } else {
-              umma_commit(&ctl->o_full[q]);
+            for (int kk = 0; kk < DP / 16; ++kk) {
+              const uint64_t off = (kk / 4) * kBlock16 + (kk % 4) * 2;
+              if (kk == 0) umma_f16_first(q * 128, qd, kd, idesc);
+              else umma_f16_more(q * 128, qd + off, kd + off, idesc);
             }
+            umma_commit(&ctl->s_full[q]);
           }
-          if (!ok) break;
-          umma_commit(&ctl->empty[v_slot]);
-          if (i + 1 < total) {
-            umma_commit(&ctl->empty[k_slot]);
+          __syncwarp();
+        };
+        // O_q += P_q V_i from the slot `from`, in two parts: the first 64 keys' probabilities are ready earlier
+        auto output = [&](int q, uint32_t& p_phase, int i, bool first, int from) {
+          const int rows = i == total - 1 ? last_rows : (i == total - 2 ? prev_rows : kTile);
+          const uint64_t vd = v_desc + from * kTile16;
+          wait(&ctl->p_ready[q][0], p_phase, 3, i);
+          if (!ok) return;
+          if (elect_one()) {
+            if (first) umma_f16_ts_first(256 + q * 128, q * 128, vd, idesc_o);
+            else umma_f16_ts_more(256 + q * 128, q * 128, vd, idesc_o);
+#pragma unroll
+            for (int kk = 1; kk < 4; ++kk)
+              if (kk * 16 < rows) umma_f16_ts_more(256 + q * 128, q * 128 + kk * 8, vd + kk * 128, idesc_o);
+          }
+          __syncwarp();
+          wait(&ctl->p_ready[q][1], p_phase, 3, i);
+          p_phase ^= 1u;
+          if (!ok) return;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 4; kk < 8; ++kk)
+              if (kk * 16 < rows) umma_f16_ts_more(256 + q * 128, q * 128 + kk * 8, vd + kk * 128, idesc_o);
+          }
+          __syncwarp();
+        };
+        auto commit = [&](uint64_t* bar) {
+          if (elect_one()) umma_commit(bar);
+          __syncwarp();
+        };
+        if (total > 0) {
+          wait(&ctl->q_full, q_phase, 1, 0);
+          q_phase ^= 1u;
+        }
+        if (!p.pair) {
+          for (int i = 0; i < 2 && i < total && ok; ++i) {
+            wait(&ctl->full[slot], phase, 2, i);
+            if (!ok) break;
+            if (i == 0) scores(0, i); else scores(1, i);
+            commit(&ctl->empty[slot]);
+            if (i + 1 == total) commit(&ctl->q_empty);
+            next();
+          }
+          auto step = [&](int q, uint32_t& p_phase, int i) {
+            wait(&ctl->full[slot], phase, 2, i);
+            if (!ok) return;
+            output(q, p_phase, i, i < 2, slot);
+            if (!ok) return;
+            commit(&ctl->empty[slot]);
+            next();
+            if (i + 2 < total) {
+              wait(&ctl->full[slot], phase, 2, i + 2);
+              if (!ok) return;
+              scores(q, i + 2);
+              commit(&ctl->empty[slot]);
+              if (i + 3 == total) commit(&ctl->q_empty);
+              next();
+            } else {
+              commit(&ctl->o_full[q]);
+            }
+          };
+          for (int i = 0; i < total && ok; i += 2) {
+            step(0, p_phase0, i);
+            if (ok && i + 1 < total) step(1, p_phase1, i + 1);
+          }
+        } else {
+          if (total > 0 && ok) wait(&ctl->full[slot], phase, 2, 0);
+          if (total > 0 && ok) {
+            if (n0 > 0) scores(0, 0);
+            if (n1 > 0) scores(1, 0);
+            commit(&ctl->empty[slot]);
+            if (total == 1) commit(&ctl->q_empty);
+            next();
+          }
+          for (int i = 0; i < total && ok; ++i) {
+            // the current slot holds V_i, the one behind it K_i+1
+            wait(&ctl->full[slot], phase, 2, i);
+            if (!ok) break;
+            const int v_slot = slot;
+            if (i + 1 < total) {
+              next();
+              wait(&ctl->full[slot], phase, 2, i + 1);
+              if (!ok) break;
+            }
+            auto step = [&](int q, uint32_t& p_phase, int tiles) {
+              if (!ok || i >= tiles) return;
+              output(q, p_phase, i, i == 0, v_slot);
+              if (!ok) return;
+              if (i + 1 < tiles) scores(q, i + 1);
+              else commit(&ctl->o_full[q]);
+            };
+            step(0, p_phase0, n0);
+            step(1, p_phase1, n1);
+            if (!ok) break;
+            commit(&ctl->empty[v_slot]);
+            if (i + 1 < total) {
+              commit(&ctl->empty[slot]);
+              if (i + 2 == total) commit(&ctl->q_empty);
+            }
             next();
           }
         }
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(&ctl->work_empty[place]);
+        if (++place == kQueue) { place = 0; place_phase ^= 1u; }
       }
-      if (!ok) {      // ... and the products in flight the time to finish
+      if (!ok) {      // leave the products in flight the time to finish
         const unsigned long long t0 = global_ns();
         while (global_ns() - t0 < 1000000ull) __nanosleep(1000);
       }
+    } else {
+      // ---------------------------------------------------------------- cleaning, and drafted keys and values
+      const int tid = threadIdx.x - 320;
+      {   // rows of no sequence: zeros, or partial results that count for nothing
+        const int64_t lo = clamp64(__ldcg(a.seqstarts), 0, a.Tq), hi = clamp64(__ldcg(a.seqstarts + a.B), lo, a.Tq);
+        const int64_t rows = (lo + a.Tq - hi) * a.Hq, step = (int64_t)gridDim.x * 2;
+        for (int64_t r = (int64_t)blockIdx.x * 2 + (tid >> 5); r < rows; r += step) {
+          const int64_t row = r < lo * a.Hq ? r : r + (hi - lo) * a.Hq;
+          if (!p.pair || p.splits == 1) {
+            T* out = reinterpret_cast<T*>(a.out) + row * a.D;
+            for (int d = lane * 8; d < a.D; d += 256) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
+          } else if (lane < p.splits) {
+            p.part_ml[(int64_t)lane * a.Tq * a.Hq + row] = make_float2(-INFINITY, 0.f);
+          }
+        }
+      }
+      uint32_t phases = 0, place_phase = 0;
+      int place = 0, entry0 = 0;
+      bool ok = true;
+      for (;;) {
+        ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->work_full[place], place_phase, ctl, 10, 0));
+        ok = !named_any(3, 64, !ok);                // the two warps leave together
+        if (!ok) break;
+        const Work& w = ctl->work[place];
+        if (w.h < 0) break;
+        const int total = tiles_of(w);
+        if (w.stores) {
+          // into the cache, where this launch does not read them
+          for (int i = tid; i < w.s.n * (a.D / 8) * 2; i += 64) {
+            const int ch = i % (a.D / 8), kv = i / (a.D / 8) & 1, t = i / (a.D / 8) >> 1;
+            const int64_t row = w.s.kv0 + w.s.len + t;
+            if (row >= a.past.rows) continue;
+            const T* src = kv ? reinterpret_cast<const T*>(a.cur.v) + (w.s.q0 + t) * a.cur.v_row + w.h * a.cur.v_head
+                              : reinterpret_cast<const T*>(a.cur.k) + (w.s.q0 + t) * a.cur.k_row + w.h * a.cur.k_head;
+            T* dst = kv ? reinterpret_cast<T*>(const_cast<void*>(a.past.v)) + row * a.past.v_row + w.h * a.past.v_head
+                        : reinterpret_cast<T*>(const_cast<void*>(a.past.k)) + row * a.past.k_row + w.h * a.past.k_head;
+            *reinterpret_cast<uint4*>(dst + ch * 8) = ld_stream16(src + ch * 8);
+          }
+        }
+        for (int i = w.partial > w.t0 ? w.partial - w.t0 : 0; i < total && ok; ++i) {
+          const int entry = 2 * i + lag < total + i ? 2 * i + lag : total + i;     // of the values of tile i
+          const int slot = (entry0 + entry) % kRing;
+          ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->raw[slot], phases >> slot & 1u, ctl, 4, i));
+          phases ^= 1u << slot;
+          const int rows = tile_rows(w, w.t0 + i), rows16 = (rows + 15) & ~15;
+          if (ok) {
+#pragma unroll
+            for (int d = 0; d < kDBlocks; ++d) {
+              uint4* at = reinterpret_cast<uint4*>(smem + (2 + slot) * kTileBytes + d * kBlockBytes);
+              for (int c = tid; c < rows16 * 8; c += 64) {
+                uint4 v = at[c];
+                uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+                if (not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w)) {
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const uint32_t bad = not_finite2<T>(e[j]);
+                    e[j] &= ~((bad >> 15) * 0xFFFFu);
+                  }
+                  at[c] = v;
+                  if (c / 8 < rows) ctl->bad[place] = w.number;
+                }
+              }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          }
+          ok = !named_any(3, 64, !ok);
+          if (ok && tid == 0) mbar_arrive(&ctl->full[slot]);
+        }
+        if (!ok) break;
+        entry0 = (entry0 + 2 * total) % kRing;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl->work_empty[place]);
+        if (++place == kQueue) { place = 0; place_phase ^= 1u; }
+      }
     }
   } else {
-    // ------------------------------------------------------------------ value tiles that some row sees a part of
-    const int tid = threadIdx.x - 320;
-    uint32_t phases = 0;
-    int first = w.partial - w.t0;
-    if (first < 0) first = 0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ------------------------------------------------------------------ softmax
+    const int half = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + lanes + half * 128, o_tmem = tmem + lanes + 256 + half * 128;
+    constexpr float kLog2e = 1.4426950408889634f;
+    // cap: c tanh(s / c) = c - 2 c / (exp(2 s / c) + 1), in log2 domain
+    const float cap2 = a.cap * kLog2e, to_cap = a.cap > 0.f ? 2.0f * kLog2e * a.scale / a.cap : 0.f;
+    const float sl2 = a.scale * kLog2e;
+    int place = 0;
+    uint32_t place_phase = 0, s_phase = 0, o_phase = 0;
     bool ok = true;
-    for (int i = first; i < total && ok; ++i) {
-      const int slot = v_entry(i) % kRing;
-      ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->raw[slot], phases >> slot & 1u, ctl, 4, i));
-      phases ^= 1u << slot;
-      const int rows = tile_rows(w, w.t0 + i), rows16 = (rows + 15) & ~15;
-      if (ok) {
+    // What a thread needs to know of its row.  Asked for anew wherever it is needed: the loop over the tiles has no register
+    // to spare for it.
+    struct Row {
+      int tok, head;
+      bool ok;
+      int64_t limit;       // keys of the past that it sees
+      uint64_t bits;       // drafted tokens that it sees
+    };
+    const int row_tok = r / p.group, row_head = r % p.group;
+    auto row_of = [&](const Work& w) {
+      asm volatile("" ::: "memory");
+      Row x;
+      x.tok = w.tok0 + (p.pair ? half * p.tokens : 0) + row_tok;
+      x.ok = r < rows_tile && x.tok < w.s.n;
+      x.head = w.h * p.group + row_head;
+      x.limit = x.ok ? visible(a, w.s, x.tok) : 0;
+      x.bits = a.tree_mask && x.ok ? (uint64_t)__ldcg(a.tree_mask + w.s.q0 + x.tok) : 0ull;
+      if (w.s.n < kTreeLimit) x.bits &= (1ull << w.s.n) - 1;           // bits behind the sequence's tokens mean nothing
+      return x;
+    };
+    for (;;) {
+      ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->work_full[place], place_phase, ctl, 11, 0));
+      if (!p.pair) ok = !named_any(4, 256, !ok);     // the two halves leave together
+      if (!ok) break;
+      const Work& w = ctl->work[place];
+      if (w.h < 0) break;
+      const int mine = p.pair ? w.nt[half] : (tiles_of(w) + 1 - half) / 2;
+      // all rows of this half see the tiles below this one whole
+      const int whole = p.pair && half && w.halves == 2 ? (int)(visible(a, w.s, w.tok0 + p.tokens) / kTile) : w.partial;
+      float slope2 = 0.f, place_of_row = 0.f;                         // SCORE: of the row among the item's keys
+      if (SCORE && a.slopes) {
+        const Row row = row_of(w);
+        if (row.ok) slope2 = __ldcg(a.slopes + row.head) * kLog2e;
+        place_of_row = (float)(row.tok + w.s.shift - (int64_t)w.t0 * kTile);
+      }
+      float m = -INFINITY, l = 0.f;                                   // m: in log2 domain
+      const int t_step = p.pair ? 1 : 2;
+      int t = w.t0 + (p.pair ? 0 : half);
+      for (int i = 0; i < mine; ++i, t += t_step) {
+        ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->s_full[half], s_phase, ctl, 5, t));
+        s_phase ^= 1u;
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t raw[128];
+        float* x = reinterpret_cast<float*>(raw);
+        uint32_t seen[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+        const bool masked = t >= whole;
+        if (masked) {
+          const Row row = row_of(w);
+          const int64_t left = row.limit - (int64_t)t * kTile;
+          const bool drafted = t == w.drafted;
 #pragma unroll
-        for (int d = 0; d < kDBlocks; ++d) {
-          uint4* at = reinterpret_cast<uint4*>(smem + (2 * kTileBytes) + slot * kTileBytes + d * kBlockBytes);
-          for (int c = tid; c < rows16 * 8; c += 64) {
-            uint4 v = at[c];
-            uint32_t* e = reinterpret_cast<uint32_t*>(&v);
-            if (not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w)) {
+          for (int k = 0; k < 4; ++k) {
+            const int n = left < 32 * k ? 0 : (left >= 32 * k + 32 ? 32 : (int)left - 32 * k);
+            seen[k] = n == 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+            if (drafted) seen[k] = k == 0 ? (uint32_t)row.bits : (k == 1 ? (uint32_t)(row.bits >> 32) : 0u);
+          }
+        }
+        float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t bad = not_finite2<T>(e[j]);
-                e[j] &= ~((bad >> 15) * 0xFFFFu);
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, raw + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_ld32(raw + 32 * c);
+          if (SCORE) {
+            if (a.cap > 0.f) {
+              // two quotients by one reciprocal of the product; 2^60 is as good as infinity here and leaves the
+              // product finite
+              float q[16];
+#pragma unroll
+              for (int j = 32 * c; j < 32 * c + 32; ++j) x[j] = min_nan(x[j] * to_cap, 60.f);
+#pragma unroll
+              for (int j = 32 * c; j < 32 * c + 32; ++j) x[j] = ex2(x[j]);
+#pragma unroll
+              for (int j = 32 * c; j < 32 * c + 32; ++j) x[j] += 1.0f;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) q[j] = rcp(x[32 * c + 2 * j] * x[32 * c + 2 * j + 1]);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float d0 = x[32 * c + 2 * j], d1 = x[32 * c + 2 * j + 1];
+                q[j] *= -2.0f * cap2;
+                x[32 * c + 2 * j] = fmaf(q[j], d1, cap2);
+                x[32 * c + 2 * j + 1] = fmaf(q[j], d0, cap2);
               }
-              at[c] = v;
-              if (c / 8 < rows) ctl->any_bad = 1;
+            } else {
+#pragma unroll
+              for (int j = 32 * c; j < 32 * c + 32; j += 2) unpair2(mul2(pair2(x[j], x[j + 1]), pair2(sl2, sl2)), x[j], x[j + 1]);
+            }
+            if (a.slopes) {
+              const float at = place_of_row - (float)((t - w.t0) * kTile);
+#pragma unroll
+              for (int j = 32 * c; j < 32 * c + 32; j += 2) {
+                const f32x2 far = pair2(fabsf(at - (float)j), fabsf(at - (float)(j + 1)));
+                unpair2(fma2(far, pair2(-slope2, -slope2), pair2(x[j], x[j + 1])), x[j], x[j + 1]);
+              }
+            }
+          }
+          if (masked) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[32 * c + j] = seen[c] & (1u << j) ? x[32 * c + j] : -INFINITY;
+          }
+#pragma unroll
+          for (int j = 32 * c; j < 32 * c + 32; j += 4) {
+            mx = max3(mx, x[j], x[j + 1]);
+            mx1 = max3(mx1, x[j + 2], x[j + 3]);
+          }
+        }
+        mx = max_nan(mx, mx1);
+        if (!SCORE) mx *= sl2;
+        // a row moves by its own maximum alone: its result does not depend on the rows beside it; NaN moves it too
+        if (i == 0) {
+          m = mx;
+        } else {
+          const bool moves = !(mx <= m + kLazy) && !(m == INFINITY);
+          if (__any_sync(0xFFFFFFFFu, moves)) {
+            const float f = moves && m != mx ? ex2(m - mx) : 1.0f;
+            m = moves ? mx : m;
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_tmem + c, o);
+              tmem_wait_ld32(o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st32(o_tmem + c, o);
             }
           }
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      }
-      ok = !named_any(3, 64, !ok);                  // the two warps leave together
-      if (ok && tid == 0) mbar_arrive(&ctl->full[slot]);
-    }
-    named_arrive(2, 320);
-  }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    // ------------------------------------------------------------------ softmax
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem + lanes + half * 128, o_tmem = tmem + lanes + 256 + half * 128;
-    const int mine = p.pair ? w.nt[half] : (total + 1 - half) / 2;
-    // all rows of this half see the tiles below this one whole
-    const int64_t first_tok = w.tok0 + (p.pair ? half * p.tokens : 0);
-    const int whole = p.pair && half && w.halves == 2 ? (int)(visible(a, w.s, first_tok) / kTile) : w.partial;
-    const int64_t limit = row_ok ? visible(a, w.s, tok) : 0;
-    uint64_t bits = a.tree_mask && row_ok ? (uint64_t)__ldcg(a.tree_mask + w.s.q0 + tok) : 0ull;
-    if (w.s.n < kTreeLimit) bits &= (1ull << w.s.n) - 1;            // bits behind the sequence's tokens mean nothing
-    constexpr float kLog2e = 1.4426950408889634f;
-    const float sl2 = SCORE ? 1.0f : a.scale * kLog2e;             // score to log2 domain, where it is not there yet
-    const float cap2 = a.cap * kLog2e, to_cap = a.cap > 0.f ? 2.0f * kLog2e * a.scale / a.cap : 0.f;
-    const float slope2 = SCORE && a.slopes && row_ok ? __ldcg(a.slopes + head) * kLog2e : 0.f;
-    float m = -INFINITY, l = 0.f;                                   // m: in log2 domain
-    bool ok = true;
-    for (int i = 0; i < mine; ++i) {
-      const int t = w.t0 + (p.pair ? i : 2 * i + half);
-      ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->s_full[half], i & 1, ctl, 5, t));
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t raw[128];
+        // -inf: nothing seen so far; +inf: inf - inf, NaN for the whole row
+        const float base = m == -INFINITY ? 0.f : (m == INFINITY ? __int_as_float(0x7FC00000) : m);
+        f32x2 sum = pair2(0.f, 0.f), sum1 = sum;
+        auto probabilities = [&](int c) {      // exponentials and sum of 32 scores, and their probabilities into tensor memory
+          const f32x2 nb = pair2(-base, -base), sc = pair2(sl2, sl2);
+          uint32_t pk[16];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, raw + c * 32);
-      tmem_wait_ld();
-      float* x = reinterpret_cast<float*>(raw);
-      if (SCORE) {
-        if (a.cap > 0.f) {
-          // c tanh(s / c) = c - 2 c / (exp(2 s / c) + 1)
-#pragma unroll
-          for (int c = 0; c < 128; ++c) x[c] = fmaf(-2.0f * cap2, rcp(ex2(x[c] * to_cap) + 1.0f), cap2);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 128; ++c) x[c] *= a.scale * kLog2e;
-        }
-        if (a.slopes) {
-          const float at = (float)(tok + w.s.shift - (int64_t)t * kTile);
-#pragma unroll
-          for (int c = 0; c < 128; ++c) x[c] = fmaf(-slope2, fabsf(at - (float)c), x[c]);
-        }
-      }
-      if (t == w.drafted) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c) x[c] = c < 64 && (bits >> (c & 63) & 1) ? x[c] : -INFINITY;
-      } else if (t >= whole) {
-        const int64_t left = limit - (int64_t)t * kTile;
-        const int n = left < 0 ? 0 : (left > kTile ? kTile : (int)left);
-#pragma unroll
-        for (int c = 0; c < 128; ++c) x[c] = c < n ? x[c] : -INFINITY;
-      }
-      float mx = x[0];
-#pragma unroll
-      for (int c = 1; c < 128; ++c) mx = fmaxf(mx, x[c]);
-      mx *= sl2;
-      if (i == 0) {
-        m = mx;
-      } else if (__any_sync(0xFFFFFFFFu, mx > m + kLazy)) {
-        // a row moves by its own maximum alone: its result does not depend on the rows beside it
-        const float next = mx > m + kLazy ? mx : m;
-        const float f = next == m ? 1.0f : ex2(m - next);
-        m = next;
-        l *= f;
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_tmem + c * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-          tmem_st32(o_tmem + c * 32, o);
-        }
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float e0 = ex2(fmaf(x[64 * c + 2 * j], sl2, -base)), e1 = ex2(fmaf(x[64 * c + 2 * j + 1], sl2, -base));
-          sum0 += e0;
-          sum1 += e1;
-          pk[j] = pack2<T>(e0, e1);
-        }
-        tmem_st32(s_tmem + c * 32, pk);
-      }
-      l += sum0 + sum1;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl->p_ready[half]);
-    }
-    // ---- the end: both halves' products are done, the smem of the ring is free
-    if (ok && mine > 0) ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->o_full[half], 0, ctl, 6, 0));
-    tc_fence_after();
-    named_sync(2, 320);
-    const bool bad = ctl->any_bad != 0;
-    // values that are not finite, of the rows this row sees in the tiles that were cleaned
-    auto add_bad = [&](float* v, int col) {
-      for (int i = w.partial > w.t0 ? w.partial - w.t0 : 0; i < total; ++i) {
-        const int t = w.t0 + i;
-        const bool draft = t == w.drafted;
-        const int rows = tile_rows(w, t);
-        for (int j = 0; j < rows; ++j) {
-          if (!(draft ? (bits >> j & 1) : (int64_t)t * kTile + j < limit)) continue;
-          const T* src = draft ? reinterpret_cast<const T*>(a.cur.v) + (w.s.q0 + j) * a.cur.v_row + w.h * a.cur.v_head
-                               : reinterpret_cast<const T*>(a.past.v) + (w.s.kv0 + (int64_t)t * kTile + j) * a.past.v_row + w.h * a.past.v_head;
-          float f[8];
-          unpack16<T>(ld_stream16(src + col), f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!isfinite(f[e])) v[e] += f[e];
-        }
-      }
-    };
-    auto store = [&](float* v, int col, float inv) {       // 8 columns of this row
-      if (!row_ok || col >= a.D) return;
-      if (bad) add_bad(v, col);
-      if (p.splits == 1) {
-        float s[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = v[e] * inv;
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + out_row * a.D + col) = pack16<T>(s);
-      } else {
-        float4* dst = reinterpret_cast<float4*>(p.part_o + ((int64_t)w.split * a.Tq * a.Hq + out_row) * a.D + col);
-        dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-        dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-      }
-    };
-    if (p.pair) {
-      if (ok && half < w.halves) {
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          if (mine > 0) {
-            tmem_ld32(o_tmem + c * 32, o);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = 0u;
+          for (int j = 0; j < 16; ++j) {
+            const f32x2 xx = pair2(x[32 * c + 2 * j], x[32 * c + 2 * j + 1]);
+            float e0, e1;
+            unpair2(SCORE ? add2(xx, nb) : fma2(xx, sc, nb), e0, e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
+            if (j & 1) sum = add2(sum, pair2(e0, e1));
+            else sum1 = add2(sum1, pair2(e0, e1));
+            pk[j] = pack2<T>(e0, e1);
           }
+          tmem_st16u(s_tmem + c * 16, pk);
+        };
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) store(reinterpret_cast<float*>(o) + j, c * 32 + j, inv);
+        for (int c = 0; c < 4; ++c) {
+          probabilities(c);
+          if (c & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ctl->p_ready[half][c >> 1]);
+          }
         }
-        if (p.splits > 1 && row_ok) p.part_ml[(int64_t)w.split * a.Tq * a.Hq + out_row] = make_float2(m, l);
+        sum = add2(sum, sum1);
+        float s0, s1;
+        unpair2(sum, s0, s1);
+        l += s0 + s1;
       }
-    } else {
-      // each half hands the other its share of the columns through shared memory, [column][row]
-      float* swap = reinterpret_cast<float*>(smem + 2 * kTileBytes);
-      float2* ml = reinterpret_cast<float2*>(swap + DP * 128);
-      ml[half * 128 + r] = make_float2(m, l);
-      uint32_t o[DP / 2];
+      // ---- the end of the item: the products of this half are done
+      if (ok && mine > 0) {
+        ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->o_full[half], o_phase, ctl, 6, w.number));
+        o_phase ^= 1u;
+      }
+      tc_fence_after();
+      const Row row = row_of(w);
+      const int total = tiles_of(w);
+      const bool row_ok = row.ok;
+      const int64_t out_row = (w.s.q0 + row.tok) * a.Hq + row.head;
+      const bool bad = ctl->bad[place] == w.number;
+      auto store = [&](Cols8& x, int col, float inv, float* part) {       // 8 columns of this row
+        if (bad) x = add_bad<T>(x, &a, &w, col, row.limit, row.bits, total);
+        if (!part) {
 #pragma unroll
-      for (int c = 0; c < DP / 64; ++c) {
-        uint32_t g[32];
-        if (mine > 0 && ok) {
-          tmem_ld32(o_tmem + (half ^ 1) * (DP / 2) + c * 32, g);
-          tmem_ld32(o_tmem + half * (DP / 2) + c * 32, o + c * 32);
-          tmem_wait_ld();
+          for (int e = 0; e < 8; ++e) x.v[e] *= inv;
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + out_row * a.D + col) = pack16<T>(x.v);
         } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) g[j] = o[c * 32 + j] = 0u;
+          reinterpret_cast<float4*>(part + col)[0] = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
+          reinterpret_cast<float4*>(part + col)[1] = make_float4(x.v[4], x.v[5], x.v[6], x.v[7]);
         }
+      };
+      if (p.pair) {
+        if (!ok) break;
+        if (half < w.halves) {
+          const float inv = l == 0.f ? 0.f : 1.0f / l;
+          float* part = nullptr;
+          if (w.slot >= 0) {
+            const int64_t at = (int64_t)w.slot * a.Tq * a.Hq + out_row;
+            part = p.part_o + at * a.D;
+            if (row_ok) p.part_ml[at] = make_float2(m, l);
+          }
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o_tmem + c, o);
+            tmem_wait_ld();
+            if (mine == 0) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) swap[((half ^ 1) * (DP / 2) + c * 32 + j) * 128 + r] = __uint_as_float(g[j]);
-      }
-      named_sync(4, 256);
-      const float2 other = ml[(half ^ 1) * 128 + r];
-      const float top = fmaxf(m, other.x);
-      const float f0 = m == -INFINITY ? 0.f : ex2(m - top), f1 = other.x == -INFINITY ? 0.f : ex2(other.x - top);
-      const float sum = l * f0 + other.y * f1;
-      const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-      if (ok) {
+              for (int j = 0; j < 32; ++j) o[j] = 0u;
+            }
 #pragma unroll
-        for (int c = 0; c < DP / 2; c += 8) {
-          float v[8];
+            for (int j = 0; j < 32; j += 8) {
+              Cols8 x;
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            v[e] = __uint_as_float(o[c + e]) * f0 + swap[(half * (DP / 2) + c + e) * 128 + r] * f1;
-          store(v, half * (DP / 2) + c, inv);
+              for (int e = 0; e < 8; ++e) x.v[e] = __uint_as_float(o[j + e]);
+              if (row_ok && c + j < a.D) store(x, c + j, inv, part);
+            }
+          }
         }
-        if (p.splits > 1 && row_ok && half == 0)
-          p.part_ml[(int64_t)w.split * a.Tq * a.Hq + out_row] = make_float2(top, sum);
+      } else {
+        // each half finishes its share of the columns; a row's lane is the same in both
+        ctl->ml[half * 128 + r] = make_float2(m, l);
+        tc_fence_before();
+        ok = !named_any(4, 256, !ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float2 other = ctl->ml[(half ^ 1) * 128 + r];
+        const float top = fmaxf(m, other.x);
+        const float f0 = m == -INFINITY ? 0.f : ex2(m - top), f1 = other.x == -INFINITY ? 0.f : ex2(other.x - top);
+        const float sum = l * f0 + other.y * f1;
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        const bool other_has = half ? total > 0 : total > 1;
+        float* part = nullptr;
+        if (w.slot >= 0) {
+          part = p.part_o + ((int64_t)w.slot * 128 + r) * a.D;
+          if (half == 0) p.part_ml[(int64_t)w.slot * 128 + r] = make_float2(top, sum);
+        }
+#pragma unroll 1
+        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+          uint32_t o[32], g[32];
+          // loaded whether there is a result or not: a conditional load would keep its 64 registers from the tile loop
+          tmem_ld32(o_tmem + c, o);
+          tmem_ld32(tmem + lanes + 256 + (half ^ 1) * 128 + c, g);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            Cols8 x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              x.v[e] = (mine > 0 ? __uint_as_float(o[j + e]) * f0 : 0.f) + (other_has ? __uint_as_float(g[j + e]) * f1 : 0.f);
+            if (row_ok && c + j < a.D) store(x, c + j, inv, part);
+          }
+        }
+        tc_fence_before();
+        named_sync(4, 256);            // both have read before the next item's products overwrite
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->work_empty[place]);
+      if (++place == kQueue) { place = 0; place_phase ^= 1u; }
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(ctl->tmem, 512);
   }
 }
 
@@ -726,18 +1067,65 @@ __global__ void __launch_bounds__(256) masked_attention_merge_kernel(const float
     acc.w = fmaf(v.w, fs, acc.w);
   }
   if (lane * 4 < D) {
-    T* dst = out + row * D + lane * 4;
-    dst[0] = Elem<T>::from_f(acc.x * inv);
-    dst[1] = Elem<T>::from_f(acc.y * inv);
-    dst[2] = Elem<T>::from_f(acc.z * inv);
-    dst[3] = Elem<T>::from_f(acc.w * inv);
+    uint2 v;
+    v.x = pack2<T>(acc.x * inv, acc.y * inv);
+    v.y = pack2<T>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(out + row * D + lane * 4) = v;
+  }
+}
+
+// The same for items whose key tiles were dealt out: one warp per row, the pieces of its item.
+template <typename T>
+__global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid_constant__ TcArgs p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const AttnArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), t = row / a.Hq;
+  if (t >= a.Tq) return;
+  int before = 0;
+  for (int i = lane; i <= a.B; i += 32) before += __ldcg(a.seqstarts + i) <= t ? 1 : 0;
+  const int b = __reduce_add_sync(0xFFFFFFFFu, before) - 1;
+  if (b < 0 || b >= a.B) return;
+  const Sequence s = load_sequence(a, b);
+  const int head = (int)(row - t * a.Hq), h = head / p.group;
+  const int64_t i = t - s.q0;
+  if (i < 0 || i >= s.n) return;
+  const int2 who = __ldcg(p.pieces + (int64_t)b * a.Hkv + h);
+  if (who.x == who.y) return;                      // in one piece: the result is there
+  const int r = (int)i * p.group + head % p.group;
+  auto slot = [&](int c) { return c == who.x ? 2 * c + 1 : 2 * c; };
+  float top = -INFINITY;
+  for (int c = who.x + lane; c <= who.y; c += 32) top = fmaxf(top, __ldcg(p.part_ml + (int64_t)slot(c) * 128 + r).x);
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  float sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = who.x; c <= who.y; ++c) {
+    const float2 ml = __ldcg(p.part_ml + (int64_t)slot(c) * 128 + r);
+    if (ml.x == -INFINITY) continue;
+    const float f = ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    if (lane * 4 < a.D) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((int64_t)slot(c) * 128 + r) * a.D) + lane);
+      acc.x = fmaf(v.x, f, acc.x);
+      acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z);
+      acc.w = fmaf(v.w, f, acc.w);
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  if (lane * 4 < a.D) {
+    uint2 v;
+    v.x = pack2<T>(acc.x * inv, acc.y * inv);
+    v.y = pack2<T>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + row * a.D + lane * 4) = v;
   }
 }
 
 // ------------------------------------------------------------------------------------------------- host side
 struct TcPlan {
   bool use;
-  int group, tokens, pair, row_blocks, splits;
+  int group, tokens, pair, row_blocks, splits, flat, grid;
 };
 
 // Everything that sizes the workspace and the grid follows from shapes and host lengths alone.
@@ -752,21 +1140,37 @@ TcPlan plan_tc(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_
   pl.tokens = kTile / pl.group;
   pl.pair = max_seqlen > pl.tokens;
   const int64_t blocks = ceil_div(max_seqlen, pl.pair ? 2 * pl.tokens : pl.tokens);
-  const int64_t ctas = blocks * B * Hkv, tiles = ceil_div(max_kvlen, kTile);
-  if (ctas > (1 << 24) || B > (1 << 20)) return pl;
+  const int64_t items = blocks * B * Hkv, tiles = ceil_div(max_kvlen, kTile) + 1;      // + 1: drafted tokens
+  if (items > (1 << 24) || B > (1 << 20)) return pl;
   pl.row_blocks = (int)blocks;
-  // Split the keys while that fills SMs that would idle, with at least 4 key tiles a CTA: below that the start of a
-  // CTA and the merge cost more than the shorter walk gains.
-  int64_t s = sm_count() / (ctas < 1 ? 1 : ctas);
-  if (s > ceil_div(tiles, 4)) s = ceil_div(tiles, 4);
-  pl.splits = (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+  const int64_t sms = sm_count();
+  int64_t grid;
+  if (pl.pair) {
+    // Split the keys while that fills SMs that would idle, with enough key tiles left for each: below that the start of an
+    // item and the merge cost more than the shorter walk gains.
+    int64_t s = sms / items;
+    if (s > tiles / kMinTiles) s = tiles / kMinTiles;
+    pl.splits = (int)(s < 1 ? 1 : (s > kMaxSplits ? kMaxSplits : s));
+    grid = items * pl.splits;
+  } else {
+    pl.splits = 1;
+    pl.flat = tiles > kMinTiles;
+    grid = pl.flat ? ceil_div(items * tiles, kMinTiles) : items;
+  }
+  pl.grid = (int)(grid < sms ? grid : sms);
   pl.use = true;
   return pl;
 }
 
-size_t tc_workspace(const TcPlan& pl, int64_t Tq, int64_t Hq, int64_t D) {
-  if (!pl.use || pl.splits == 1) return 0;
-  return (size_t)pl.splits * Tq * Hq * ((size_t)D * sizeof(float) + sizeof(float2));
+// 16-byte aligned parts: maximum and sum, results, and who shares an item
+size_t tc_workspace(const TcPlan& pl, int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, size_t* o_at = nullptr,
+                    size_t* pieces_at = nullptr) {
+  if (!pl.use || (pl.splits == 1 && !pl.flat)) return 0;
+  const size_t rows = pl.flat ? (size_t)pl.grid * 2 * kTile : (size_t)pl.splits * Tq * Hq;
+  const size_t o = (rows * sizeof(float2) + 15) & ~(size_t)15, pieces = o + rows * D * sizeof(float);
+  if (o_at) *o_at = o;
+  if (pieces_at) *pieces_at = pieces;
+  return pieces + (pl.flat ? (size_t)B * Hkv * sizeof(int2) : 0);
 }
 
 bool rows_ok_for_tma(const void* base, int64_t row, int64_t head, int64_t rows) {
@@ -791,18 +1195,20 @@ int make_head_map(CUtensorMap* map, const void* base, int64_t rows, int heads, i
 }
 
 template <typename T, int DP>
-int launch_tc_t(const TileMaps& maps, const TcArgs& p, cudaStream_t s) {
+int launch_tc_t(const TileMaps& maps, const TcArgs& p, int grid, cudaStream_t s) {
   const bool score = p.a.cap > 0.f || p.a.slopes;
   const void* kern = score ? (const void*)masked_attention_kernel<T, DP, true> : (const void*)masked_attention_kernel<T, DP, false>;
-  const size_t smem = (size_t)(2 + kRing) * kTile * DP * 2 + sizeof(Ctl) + 1024;
+  const size_t smem = (size_t)(2 + kRing) * kTile * DP * 2 + sizeof(Ctl);
+  static_assert((2 + kRing) * kTile * DP * 2 + sizeof(Ctl) <= 227 * 1024, "shared memory of an SM");
   PMX_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  const int64_t grid = (int64_t)p.row_blocks * p.a.B * p.a.Hkv * p.splits + p.zero_ctas;
   void* args[] = {(void*)&maps, (void*)&p};
   const int st = launch_pdl(kern, dim3((unsigned)grid), dim3(kAttnThreads), smem, s, args);
-  if (st != PMX_OK || p.splits == 1) return st;
+  if (st != PMX_OK || (p.splits == 1 && !p.flat)) return st;
   const int64_t rows = p.a.Tq * p.a.Hq;
-  return launch_pdl_k(masked_attention_merge_kernel<T>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, s,
-                      (const float*)p.part_o, (const float2*)p.part_ml, (T*)p.a.out, rows, p.a.D, p.splits);
+  const dim3 merge_grid((unsigned)ceil_div(rows, 8)), merge_block(256);
+  if (p.flat) return launch_pdl_k(masked_attention_join_kernel<T>, merge_grid, merge_block, 0, s, p);
+  return launch_pdl_k(masked_attention_merge_kernel<T>, merge_grid, merge_block, 0, s, (const float*)p.part_o,
+                      (const float2*)p.part_ml, (T*)p.a.out, rows, p.a.D, p.splits);
 }
 
 // Runs the call on the tensor cores if they cover it (*done), otherwise leaves it to the row kernel.
@@ -819,9 +1225,12 @@ int launch_tc(const AttnArgs& a, const TcPlan& pl, int dtype, const char* name, 
   TcArgs p{};
   p.a = a;
   p.group = pl.group; p.tokens = pl.tokens; p.row_blocks = pl.row_blocks; p.splits = pl.splits; p.pair = pl.pair;
-  p.zero_ctas = (int)(a.Tq / 512 < 1 ? 1 : (a.Tq / 512 > 32 ? 32 : a.Tq / 512));
+  p.flat = pl.flat;
+  size_t o_at = 0, pieces_at = 0;
+  tc_workspace(pl, a.Tq, a.B, a.Hq, a.Hkv, a.D, &o_at, &pieces_at);
   p.part_ml = reinterpret_cast<float2*>(ws);
-  p.part_o = reinterpret_cast<float*>(p.part_ml + (size_t)pl.splits * a.Tq * a.Hq);
+  p.part_o = reinterpret_cast<float*>((char*)ws + o_at);
+  p.pieces = reinterpret_cast<int2*>((char*)ws + pieces_at);
   TileMaps m{};
   int st = make_head_map(&m.q, a.q, a.Tq, a.Hq, a.D, a.q_tok, a.q_head, (uint32_t)pl.group, (uint32_t)pl.tokens, dtype, name);
   if (st == PMX_OK) st = make_head_map(&m.k, a.past.k, a.past.rows, a.Hkv, a.D, a.past.k_row, a.past.k_head, 1, kTile, dtype, name);
@@ -830,6 +1239,6 @@ int launch_tc(const AttnArgs& a, const TcPlan& pl, int dtype, const char* name, 
   if (st == PMX_OK && a.tree_mask) st = make_head_map(&m.cv, a.cur.v, a.cur.rows, a.Hkv, a.D, a.cur.v_row, a.cur.v_head, 1, kTreeLimit, dtype, name);
   if (st != PMX_OK) return st;
   const bool bf = dtype == PMX_DTYPE_BF16;
-  if (a.D <= 64) return bf ? launch_tc_t<__nv_bfloat16, 64>(m, p, s) : launch_tc_t<__half, 64>(m, p, s);
-  return bf ? launch_tc_t<__nv_bfloat16, 128>(m, p, s) : launch_tc_t<__half, 128>(m, p, s);
+  if (a.D <= 64) return bf ? launch_tc_t<__nv_bfloat16, 64>(m, p, pl.grid, s) : launch_tc_t<__half, 64>(m, p, pl.grid, s);
+  return bf ? launch_tc_t<__nv_bfloat16, 128>(m, p, pl.grid, s) : launch_tc_t<__half, 128>(m, p, pl.grid, s);
 }
