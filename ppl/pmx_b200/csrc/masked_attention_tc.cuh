@@ -80,14 +80,17 @@ struct Ctl {
   volatile int abort;
 };
 
+// The clock is read only after many polls: reading %globaltimer takes long, and a wait that ends meanwhile would be
+// noticed late.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* c, int role, int tile) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = global_ns();
+  unsigned long long t0 = 0;
   for (uint32_t it = 1;; ++it) {
     if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 63u) == 0u) {
+    if ((it & 127u) == 0u) {
       if (c->abort) return false;
-      if (global_ns() - t0 > kAttnWaitNs) {
+      const unsigned long long now = global_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kAttnWaitNs) {
         c->abort = 1;
         if (atomicExch(&g_attention_status[0], 1) != 1) {
           g_attention_status[1] = role;
@@ -565,42 +568,62 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
           ok = __all_sync(0xFFFFFFFFu, wait_bar(bar, parity, ctl, role, i));
           tc_fence_after();
         };
-        // S_q = Q_q K_i^T from the current slot
-        auto scores = [&](int q, int i) {
-          if (elect_one()) {
-            const uint64_t kd = k_desc + slot * kTile16, qd = q_desc + (p.pair ? q : 0) * kTile16;
-            const uint32_t idesc = i == drafted ? idesc_d : idesc_s;
+        // What an elected lane issues, without a branch where the tile is full:
+        // S_q = Q_q K_i^T with the keys in slot `from`
+        auto issue_scores = [&](int q, int i, int from) {
+          const uint64_t kd = k_desc + from * kTile16, qd = q_desc + (p.pair ? q : 0) * kTile16;
+          const uint32_t idesc = i == drafted ? idesc_d : idesc_s;
+          umma_f16_first(q * 128, qd, kd, idesc);
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-              const uint64_t off = (kk / 4) * kBlock16 + (kk % 4) * 2;
-              if (kk == 0) umma_f16_first(q * 128, qd, kd, idesc);
-              else umma_f16_more(q * 128, qd + off, kd + off, idesc);
-            }
-            umma_commit(&ctl->s_full[q]);
+          for (int kk = 1; kk < DP / 16; ++kk) {
+            const uint64_t off = (kk / 4) * kBlock16 + (kk % 4) * 2;
+            umma_f16_more(q * 128, qd + off, kd + off, idesc);
           }
+          umma_commit(&ctl->s_full[q]);
+        };
+        // O_q += P_q V for the 64 keys of one half of the tile in slot `from`, of which `rows` exist
+        auto issue_output = [&](int q, int from, int upper, int rows, bool first) {
+          const uint64_t vd = v_desc + from * kTile16 + upper * 512;
+          const uint32_t pt = q * 128 + upper * 32, ot = 256 + q * 128;
+          rows -= upper * 64;
+          if (rows > 48) {
+            if (first) umma_f16_ts_first(ot, pt, vd, idesc_o);
+            else umma_f16_ts_more(ot, pt, vd, idesc_o);
+            umma_f16_ts_more(ot, pt + 8, vd + 128, idesc_o);
+            umma_f16_ts_more(ot, pt + 16, vd + 256, idesc_o);
+            umma_f16_ts_more(ot, pt + 24, vd + 384, idesc_o);
+          } else {
+            for (int kk = 0; kk * 16 < rows; ++kk) {
+              if (first && kk == 0) umma_f16_ts_first(ot, pt, vd, idesc_o);
+              else umma_f16_ts_more(ot, pt + kk * 8, vd + kk * 128, idesc_o);
+            }
+          }
+        };
+        auto scores = [&](int q, int i) {
+          if (elect_one()) issue_scores(q, i, slot);
           __syncwarp();
         };
-        // O_q += P_q V_i from the slot `from`, in two parts: the first 64 keys' probabilities are ready earlier
-        auto output = [&](int q, uint32_t& p_phase, int i, bool first, int from) {
+        // One tile of one half: the products with its probabilities (the first 64 keys' are ready earlier), then the scores
+        // of the half's next tile, if `next_i` >= 0, from slot `k_slot`; `frees`: slots that nothing needs after this.
+        auto step = [&](int q, uint32_t& p_phase, int i, bool first, int v_slot, int next_i, int k_slot, bool frees,
+                        bool last_scores) {
           const int rows = i == total - 1 ? last_rows : (i == total - 2 ? prev_rows : kTile);
-          const uint64_t vd = v_desc + from * kTile16;
           wait(&ctl->p_ready[q][0], p_phase, 3, i);
           if (!ok) return;
-          if (elect_one()) {
-            if (first) umma_f16_ts_first(256 + q * 128, q * 128, vd, idesc_o);
-            else umma_f16_ts_more(256 + q * 128, q * 128, vd, idesc_o);
-#pragma unroll
-            for (int kk = 1; kk < 4; ++kk)
-              if (kk * 16 < rows) umma_f16_ts_more(256 + q * 128, q * 128 + kk * 8, vd + kk * 128, idesc_o);
-          }
+          if (elect_one()) issue_output(q, v_slot, 0, rows, first);
           __syncwarp();
           wait(&ctl->p_ready[q][1], p_phase, 3, i);
           p_phase ^= 1u;
           if (!ok) return;
           if (elect_one()) {
-#pragma unroll
-            for (int kk = 4; kk < 8; ++kk)
-              if (kk * 16 < rows) umma_f16_ts_more(256 + q * 128, q * 128 + kk * 8, vd + kk * 128, idesc_o);
+            issue_output(q, v_slot, 1, rows, false);
+            if (next_i >= 0) issue_scores(q, next_i, k_slot);
+            else umma_commit(&ctl->o_full[q]);
+            if (frees) {
+              umma_commit(&ctl->empty[v_slot]);
+              if (k_slot != v_slot) umma_commit(&ctl->empty[k_slot]);
+              if (last_scores) umma_commit(&ctl->q_empty);
+            }
           }
           __syncwarp();
         };
@@ -621,27 +644,22 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
             if (i + 1 == total) commit(&ctl->q_empty);
             next();
           }
-          auto step = [&](int q, uint32_t& p_phase, int i) {
+          auto turn = [&](int q, uint32_t& p_phase, int i) {
             wait(&ctl->full[slot], phase, 2, i);
             if (!ok) return;
-            output(q, p_phase, i, i < 2, slot);
-            if (!ok) return;
-            commit(&ctl->empty[slot]);
-            next();
-            if (i + 2 < total) {
+            const int v_slot = slot;
+            const bool more = i + 2 < total;
+            if (more) {
+              next();
               wait(&ctl->full[slot], phase, 2, i + 2);
               if (!ok) return;
-              scores(q, i + 2);
-              commit(&ctl->empty[slot]);
-              if (i + 3 == total) commit(&ctl->q_empty);
-              next();
-            } else {
-              commit(&ctl->o_full[q]);
             }
+            step(q, p_phase, i, i < 2, v_slot, more ? i + 2 : -1, slot, true, i + 3 == total);
+            next();
           };
           for (int i = 0; i < total && ok; i += 2) {
-            step(0, p_phase0, i);
-            if (ok && i + 1 < total) step(1, p_phase1, i + 1);
+            turn(0, p_phase0, i);
+            if (ok && i + 1 < total) turn(1, p_phase1, i + 1);
           }
         } else {
           if (total > 0 && ok) wait(&ctl->full[slot], phase, 2, 0);
@@ -652,32 +670,25 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
             if (total == 1) commit(&ctl->q_empty);
             next();
           }
-          for (int i = 0; i < total && ok; ++i) {
-            // the current slot holds V_i, the one behind it K_i+1
+          // V_i and, behind it, K_i+1 are waited for one step ahead, between the two halves: what follows a half's last
+          // product delays the other half's first one
+          int v_slot = slot, k_slot = slot;
+          auto fetched = [&](int i) {
             wait(&ctl->full[slot], phase, 2, i);
-            if (!ok) break;
-            const int v_slot = slot;
-            if (i + 1 < total) {
-              next();
-              wait(&ctl->full[slot], phase, 2, i + 1);
-              if (!ok) break;
-            }
-            auto step = [&](int q, uint32_t& p_phase, int tiles) {
-              if (!ok || i >= tiles) return;
-              output(q, p_phase, i, i == 0, v_slot);
-              if (!ok) return;
-              if (i + 1 < tiles) scores(q, i + 1);
-              else commit(&ctl->o_full[q]);
-            };
-            step(0, p_phase0, n0);
-            step(1, p_phase1, n1);
-            if (!ok) break;
-            commit(&ctl->empty[v_slot]);
-            if (i + 1 < total) {
-              commit(&ctl->empty[slot]);
-              if (i + 2 == total) commit(&ctl->q_empty);
-            }
+            v_slot = k_slot = slot;
             next();
+            if (ok && i + 1 < total) {
+              wait(&ctl->full[slot], phase, 2, i + 1);
+              k_slot = slot;
+              next();
+            }
+          };
+          if (total > 0 && ok) fetched(0);
+          for (int i = 0; i < total && ok; ++i) {
+            const int v = v_slot, k = k_slot;
+            if (i < n0) step(0, p_phase0, i, i == 0, v, i + 1 < n0 ? i + 1 : -1, k, n1 == 0, i + 2 == total);
+            if (ok && i + 1 < total) fetched(i + 1);
+            if (ok && i < n1) step(1, p_phase1, i, i == 0, v, i + 1 < n1 ? i + 1 : -1, k, true, i + 2 == total);
           }
         }
         if (!ok) break;
