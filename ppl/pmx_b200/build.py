@@ -10,6 +10,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libpmx_moe_b200.so")
+HOST = os.path.join(PKG, "_host_calls.so")       # the regular case of some operators' host side (csrc/host_calls.cpp)
 SOURCES = ["cabi.cu", "select.cu", "elementwise.cu", "gemm_simt.cu", "gemm_tcgen05.cu", "gemm_tcgen05_pair.cu", "combine_allreduce.cu", "attention.cu", "mlp_tcgen05.cu",
            "rotary.cu", "cache_rows.cu", "masked_attention.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -23,21 +24,33 @@ def _nvcc() -> str:
 
 
 def _stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(HOST):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(PKG, "..", "..", "include", "pmx_moe.h"))
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _host_command() -> list:
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    inc = [f"-I{d}" for d in (*cpp_extension.include_paths(), cuda, sysconfig.get_paths()["include"])]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *inc, os.path.join(CSRC, "host_calls.cpp"), "-o", HOST, f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch_python"]
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every .cu of csrc/ into one shared library; returns its path."""
+    """Compile every .cu of csrc/ into one shared library, and the host calls beside it; returns the library's path."""
     if not force and not _stale():
         return LIB
     nvcc = _nvcc()
     objs = []
-    procs = []
+    procs = [("host_calls.cpp", subprocess.Popen(_host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))]
     for src in SOURCES:
         obj = os.path.join(CSRC, src[:-3] + ".o")
         cmd = [nvcc, *ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",

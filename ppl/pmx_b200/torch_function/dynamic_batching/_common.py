@@ -2,8 +2,19 @@
 from __future__ import annotations
 
 import contextlib
+import ctypes as C
 
 import torch
+
+from ..._cabi import lib
+
+try:
+    from ... import _host_calls as host
+except ImportError as e:
+    raise ImportError("ppl/pmx_b200/_host_calls.so cannot be loaded: build it with `python -m ppl.pmx_b200.build`") from e
+host.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+    "pmx_rotary_embedding", "pmx_prompt_attention", "pmx_tree_cache_attention", "pmx_compact_cache",
+    "pmx_attention_workspace_bytes")))
 
 _NULL = contextlib.nullcontext()
 # the raw stream handle and the current device without the objects that torch.cuda wraps them in: these
@@ -14,6 +25,9 @@ raw_stream = torch._C._cuda_getCurrentRawStream
 def on_device(index: int):
     """Makes device `index` current for a launch; free when it is already."""
     return _NULL if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+is_tracing = torch.jit.is_tracing
 
 
 def exporting() -> bool:

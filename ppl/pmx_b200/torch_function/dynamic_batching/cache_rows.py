@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from ..._cabi import lib, check, COMPACT_CACHE_ARGS, DTYPE_CODE
-from ._common import cache_strides, host_int, index, on_device, raw_stream, same_device
+from ._common import cache_strides, host, host_int, index, on_device, raw_stream, same_device
 
 
 def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: torch.Tensor, accept_starts: torch.Tensor,
@@ -16,6 +16,10 @@ def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: tor
     base = cachestarts[b] + start_pos[b], in all layers, keys and values.  All rows of a sequence are read before one is
     written, so the indices may come in any order and repeat; a negative index leaves its row alone.  The caller's next
     start_pos is start_pos + the number accepted.  Rows of different sequences must not overlap."""
+    status = host.compact(cache, cachestarts, start_pos, accept_starts, accept_index, max_accept, num_layer, cache_layout)
+    if status is not None:           # None: not the regular case
+        check(status)
+        return cache
     name = "compact_cache"
     dev = cache.get_device()
     for t in (cache, cachestarts, start_pos, accept_starts, accept_index):

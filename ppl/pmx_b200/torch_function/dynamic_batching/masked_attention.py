@@ -15,8 +15,8 @@ from typing import Optional
 import torch
 
 from ..._cabi import lib, check, workspace, DTYPE_CODE, PROMPT_ATTENTION_ARGS, TREE_ATTENTION_ARGS
-from ._common import (cache_strides, exporting, heads, host_int, index, on_device, raw_stream, same_device,
-                      wants_grad)
+from ._common import (cache_strides, exporting, heads, host, host_int, index, is_tracing, on_device, raw_stream,
+                      same_device, wants_grad)
 
 
 
@@ -204,6 +204,10 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     query, key and value may be views with unit inner stride.  float16, bfloat16, float32, head_dim up to 256."""
     args = (query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_heads, head_dim, is_causal, num_kv_heads,
             scale, float(logit_cap), alibi_slopes, prefix_lens)
+    if not is_tracing():
+        out = host.prompt(*args)
+        if out is not None:          # None: not the regular case
+            return out if type(out) is not int else check(out)
     if exporting() or wants_grad(query, key, value, alibi_slopes):
         return PromptAttention.apply(*args)
     return _prompt(*args)
@@ -225,6 +229,10 @@ def tree_cache_attention(query: torch.Tensor, current_key: torch.Tensor, current
     prompt_attention()."""
     args = (query, current_key, current_value, seqstarts, cachestarts, start_pos, tree_mask, max_seqlen, max_kvlen, cache,
             num_heads, head_dim, num_kv_heads, num_layer, layer_idx, cache_layout, scale, float(logit_cap))
+    if not is_tracing():
+        out = host.tree(*args)
+        if out is not None:          # None: not the regular case
+            return out if type(out) is not int else check(out)
     if exporting() or wants_grad(query, current_key, current_value, cache):
         return TreeCacheAttention.apply(*args)
     return _tree(*args)

@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from ..._cabi import lib, check, DTYPE_CODE, ROTARY_ARGS
-from ._common import exporting, heads, index, on_device, raw_stream, same_device, wants_grad
+from ._common import exporting, heads, host, index, is_tracing, on_device, raw_stream, same_device, wants_grad
 
 
 @functools.lru_cache(maxsize=64)
@@ -182,6 +182,13 @@ def rotary_position_embedding(query: torch.Tensor, key: Optional[torch.Tensor], 
     start_pos[b] + t - seqstarts[b], or at position_ids[t] where those are given (drafted trees: the depth).
     Tokens of no sequence are copied.  Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) when `interleaved`;
     `scaling_type` as in rotary_frequencies().  float16, bfloat16, float32; one rounding of the result."""
+    if not is_tracing():
+        r = rotary_dim or query.shape[-1]
+        _, table, factor = _table(r, theta, scaling_type, scaling_factor, original_max_position)
+        out = host.rotary(query, key, None, None, 0.0, seqstarts, start_pos, position_ids, r, 1 if interleaved else 0, table,
+                          factor)
+        if out is not None:          # None: not the regular case
+            return out if type(out) is tuple else check(out)
     args = (query, key, seqstarts, start_pos, position_ids, rotary_dim, theta, interleaved, scaling_type,
             scaling_factor, original_max_position)
     if exporting() or wants_grad(query, key):
@@ -201,6 +208,13 @@ def qk_norm_rotary_embedding(query: torch.Tensor, key: torch.Tensor, query_norm_
     one for all key heads), then the rotation; one rounding at the end."""
     if query_norm_weight is None or key_norm_weight is None or key is None:
         raise ValueError("qk_norm_rotary_embedding: key and both norm weights are needed")
+    if not is_tracing():
+        r = rotary_dim or query.shape[-1]
+        _, table, factor = _table(r, theta, scaling_type, scaling_factor, original_max_position)
+        out = host.rotary(query, key, query_norm_weight, key_norm_weight, float(eps), seqstarts, start_pos, position_ids, r,
+                          1 if interleaved else 0, table, factor)
+        if out is not None:
+            return out if type(out) is tuple else check(out)
     args = (query, key, query_norm_weight, key_norm_weight, float(eps), seqstarts, start_pos, position_ids, rotary_dim,
             theta, interleaved, scaling_type, scaling_factor, original_max_position)
     if exporting() or wants_grad(query, key, query_norm_weight, key_norm_weight):

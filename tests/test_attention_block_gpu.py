@@ -529,3 +529,36 @@ def test_prompt_then_a_speculative_step_equals_the_long_prompt(DB, dtype):
     got = torch.cat([torch.cat([first[s0[b]:s0[b + 1]], second[s1[b]:s1[b + 1]][path[b]], third[b:b + 1]]) for b in range(B)])
     # two results of the same sums, each with its probabilities and its result rounded once (values up to ~4)
     assert (got.float() - want.float()).abs().max() <= 4 * UNIT[dtype] * float(want.float().abs().max())
+
+
+def test_calls_that_need_converting_give_the_same_as_regular_ones(DB):
+    """Regular calls take a short way through the host (host_calls.cpp); index arrays of 32 bits, lengths as tensors,
+    strided arrays and parameters take the general one."""
+    rng = np.random.default_rng(12)
+    T, Hq, Hkv, D = 40, 4, 2, 64
+    x = dev(values(rng, (T, Hq + 2 * Hkv, D), "bf16"), "bf16")
+    q, k, v, w = x[:, :Hq], x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:], torch.ones(D, device="cuda", dtype=torch.bfloat16)
+    ss, sp = i64([0, 15, 40]), i64([3, 0])
+    wide = torch.stack([ss, ss], 1)[:, 0]                       # the same values with a stride
+    one = lambda n: torch.tensor([n])                           # noqa: E731
+    eq = lambda a, b: all(torch.equal(m, n) for m, n in zip(a, b))  # noqa: E731
+    want = DB.rotary_position_embedding(q, k, ss, sp)
+    assert eq(DB.rotary_position_embedding(q, k, ss.int(), sp), want) and eq(DB.rotary_position_embedding(q, k, wide, sp.int()), want)
+    want = DB.qk_norm_rotary_embedding(q, k, w, w, 1e-6, ss, sp)
+    assert eq(DB.qk_norm_rotary_embedding(q, k, torch.nn.Parameter(w, False), w, 1e-6, ss, sp.int()), want)
+    args = dict(num_kv_heads=Hkv, logit_cap=20.0, prefix_lens=i64([4, 9]), alibi_slopes=torch.full((Hq,), 0.25, device="cuda"))
+    want = DB.prompt_attention(q, k, v, ss, ss, 25, 25, Hq, D, **args)
+    assert torch.equal(DB.prompt_attention(q, k, v, wide, ss.int(), one(25), one(25), Hq, D, **args), want)
+    assert torch.equal(DB.prompt_attention(q, k, v, ss, ss, 25, 25, Hq, D, **{**args, "alibi_slopes": args["alibi_slopes"].double()}), want)
+    caches = [dev(cache_of(np.random.default_rng(3), 1, 90, 2, Hkv, D, "bf16"), "bf16") for _ in range(2)]
+    mask = i64([-1] * T)
+    outs = [DB.tree_cache_attention(q, k, v, s, i64([0, 40]), sp, mask, m, n, c, Hq, D, num_kv_heads=Hkv, num_layer=2, layer_idx=1,
+                                    cache_layout=1) for c, s, m, n in zip(caches, (ss, ss.int()), (25, one(25)), (40, one(40)))]
+    assert eq(outs, outs[::-1]) and torch.equal(*caches)
+    for c, s, m in zip(caches, (i64([0, 2, 5]), i64([0, 2, 5]).int()), (3, one(3))):
+        DB.compact_cache(c, i64([0, 40]), sp, s, i64([1, 4, 3, 0, 24]), m, num_layer=2, cache_layout=1)
+    assert torch.equal(*caches)
+    with torch.no_grad():                                       # a gradient that nobody asks for
+        assert eq(DB.rotary_position_embedding(q.clone().requires_grad_(), k, ss, sp), DB.rotary_position_embedding(q, k, ss, sp))
+    with pytest.raises(Exception, match="backward|derivative|grad"):
+        DB.rotary_position_embedding(q.clone().requires_grad_(), k, ss, sp)[0].sum().backward()
