@@ -231,6 +231,17 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// tanh(y) / y of two values in [-1, 1]: a polynomial of degree 6 in y^2 whose largest relative error is least (weighted
+// least squares iterated to equal ripples: 5.0e-8, 1.7e-7 with the roundings)
+__device__ __forceinline__ f32x2 tanh_over_y(f32x2 y) {
+  const f32x2 z = mul2(y, y);
+  f32x2 p = fma2(z, pair2(0x1.10e5d0p-10f, 0x1.10e5d0p-10f), pair2(-0x1.968b68p-8f, -0x1.968b68p-8f));
+  p = fma2(p, z, pair2(0x1.4c6e56p-6f, 0x1.4c6e56p-6f));
+  p = fma2(p, z, pair2(-0x1.b5eb84p-5f, -0x1.b5eb84p-5f));
+  p = fma2(p, z, pair2(0x1.10e672p-3f, 0x1.10e672p-3f));
+  p = fma2(p, z, pair2(-0x1.55540ap-2f, -0x1.55540ap-2f));
+  return fma2(p, z, pair2(0x1.fffffep-1f, 0x1.fffffep-1f));
+}
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -421,7 +432,7 @@ __device__ __noinline__ Cols8 add_bad(Cols8 x, const AttnArgs* ap, const Work* w
   return x;
 }
 
-template <typename T, int DP, bool SCORE>
+template <typename T, int DP>
 __global__ void __launch_bounds__(kAttnThreads, 1)
 masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TcArgs p) {
   constexpr int kTileBytes = kTile * DP * 2;
@@ -781,9 +792,10 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + half * 128, o_tmem = tmem + lanes + 256 + half * 128;
     constexpr float kLog2e = 1.4426950408889634f;
-    // cap: c tanh(s / c) = c - 2 c / (exp(2 s / c) + 1), in log2 domain
-    const float cap2 = a.cap * kLog2e, to_cap = a.cap > 0.f ? 2.0f * kLog2e * a.scale / a.cap : 0.f;
+    const float cap2 = a.cap * kLog2e, to_y = a.cap > 0.f ? a.scale / a.cap : 0.f;      // cap in log2 domain; s / c of a product
     const float sl2 = a.scale * kLog2e;
+    const bool score = a.cap > 0.f || a.slopes;       // scores are rewritten, in log2 domain then
+    const float sl = score ? 1.0f : sl2;
     int place = 0;
     uint32_t place_phase = 0, s_phase = 0, o_phase = 0;
     bool ok = true;
@@ -807,6 +819,83 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
       if (w.s.n < kTreeLimit) x.bits &= (1ull << w.s.n) - 1;           // bits behind the sequence's tokens mean nothing
       return x;
     };
+    // Cap, distance bias and mask: the scores of a tile as they have to be, written back to tensor memory.  A pass of its own
+    // in a loop that is not unrolled, run only where there is something to do: the hot loop is as long as the instruction
+    // caches can bear (the same arithmetic inside it, unrolled, took 1184 us where this takes 961, and code that
+    // was merely skipped cost a fifth).
+    auto adjust = [&](const Work& w, int t, int whole, float slope2, float place_of_row) {
+      uint32_t seen[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
+      if (t >= whole) {
+        const Row row = row_of(w);
+        const int64_t left = row.limit - (int64_t)t * kTile;
+        const bool drafted = t == w.drafted;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int n = left < 32 * k ? 0 : (left >= 32 * k + 32 ? 32 : (int)left - 32 * k);
+          seen[k] = n == 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+          if (drafted) seen[k] = k == 0 ? (uint32_t)row.bits : (k == 1 ? (uint32_t)(row.bits >> 32) : 0u);
+        }
+      }
+      const f32x2 sc = a.cap > 0.f || !score ? pair2(1.f, 1.f) : pair2(sl2, sl2);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t raw[32];
+        float* x = reinterpret_cast<float*>(raw);
+        tmem_ld32(s_tmem + c * 32, raw);
+        tmem_wait_ld32(raw);
+        if (a.cap > 0.f) {
+          float big = 0.f;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) big = max3(big, fabsf(x[j]), fabsf(x[j + 1]));
+          if (__all_sync(0xFFFFFFFFu, big * to_y <= 1.0f)) {
+            // |s| <= c, as almost everywhere: tanh by its polynomial, off the special function unit
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const f32x2 xx = pair2(x[j], x[j + 1]);
+              unpair2(mul2(mul2(xx, pair2(sl2, sl2)), tanh_over_y(mul2(xx, pair2(to_y, to_y)))), x[j], x[j + 1]);
+            }
+          } else {
+            // c - 2 c / (exp(2 s / c) + 1), two quotients by one reciprocal of the product; 2^60 is as good as
+            // infinity here and leaves the product finite
+            const float to_cap = 2.0f * kLog2e * to_y;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float d0 = ex2(min_nan(x[j] * to_cap, 60.f)) + 1.0f, d1 = ex2(min_nan(x[j + 1] * to_cap, 60.f)) + 1.0f;
+              const float q = rcp(d0 * d1) * (-2.0f * cap2);
+              x[j] = fmaf(q, d1, cap2);
+              x[j + 1] = fmaf(q, d0, cap2);
+            }
+          }
+        }
+        if (a.slopes) {
+          const float at = place_of_row - (float)((t - w.t0) * kTile + 32 * c);
+          if (__all_sync(0xFFFFFFFFu, at >= 31.f)) {
+            // all 32 keys lie before all rows: the bias climbs by the slope from key to key
+            f32x2 b0 = pair2(-slope2 * at, -slope2 * (at - 1.f)), b1 = pair2(-slope2 * (at - 2.f), -slope2 * (at - 3.f));
+            const f32x2 up = pair2(4.f * slope2, 4.f * slope2);
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+              unpair2(fma2(pair2(x[j], x[j + 1]), sc, b0), x[j], x[j + 1]);
+              unpair2(fma2(pair2(x[j + 2], x[j + 3]), sc, b1), x[j + 2], x[j + 3]);
+              b0 = add2(b0, up);
+              b1 = add2(b1, up);
+            }
+          } else {
+            const float one = a.cap > 0.f ? 1.0f : sl2;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = fmaf(-slope2, fabsf(at - (float)j), x[j] * one);
+          }
+        }
+        const uint32_t bits = c < 2 ? (c == 0 ? seen[0] : seen[1]) : (c == 2 ? seen[2] : seen[3]);
+        if (bits != 0xFFFFFFFFu) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] = bits & (1u << j) ? x[j] : -INFINITY;
+        }
+        __syncwarp();
+        tmem_st32(s_tmem + c * 32, raw);
+      }
+      tmem_wait_st();
+    };
     for (;;) {
       ok = __all_sync(0xFFFFFFFFu, wait_bar(&ctl->work_full[place], place_phase, ctl, 11, 0));
       if (!p.pair) ok = !named_any(4, 256, !ok);     // the two halves leave together
@@ -816,8 +905,8 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
       const int mine = p.pair ? w.nt[half] : (tiles_of(w) + 1 - half) / 2;
       // all rows of this half see the tiles below this one whole
       const int whole = p.pair && half && w.halves == 2 ? (int)(visible(a, w.s, w.tok0 + p.tokens) / kTile) : w.partial;
-      float slope2 = 0.f, place_of_row = 0.f;                         // SCORE: of the row among the item's keys
-      if (SCORE && a.slopes) {
+      float slope2 = 0.f, place_of_row = 0.f;                         // of the row; its place among the item's keys
+      if (a.slopes) {
         const Row row = row_of(w);
         if (row.ok) slope2 = __ldcg(a.slopes + row.head) * kLog2e;
         place_of_row = (float)(row.tok + w.s.shift - (int64_t)w.t0 * kTile);
@@ -830,73 +919,22 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         s_phase ^= 1u;
         if (!ok) break;
         tc_fence_after();
+        if (score || t >= whole) adjust(w, t, whole, slope2, place_of_row);
         uint32_t raw[128];
         float* x = reinterpret_cast<float*>(raw);
-        uint32_t seen[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
-        const bool masked = t >= whole;
-        if (masked) {
-          const Row row = row_of(w);
-          const int64_t left = row.limit - (int64_t)t * kTile;
-          const bool drafted = t == w.drafted;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int n = left < 32 * k ? 0 : (left >= 32 * k + 32 ? 32 : (int)left - 32 * k);
-            seen[k] = n == 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
-            if (drafted) seen[k] = k == 0 ? (uint32_t)row.bits : (k == 1 ? (uint32_t)(row.bits >> 32) : 0u);
-          }
-        }
-        float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, raw + 32 * c);
+        float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           tmem_wait_ld32(raw + 32 * c);
-          if (SCORE) {
-            if (a.cap > 0.f) {
-              // two quotients by one reciprocal of the product; 2^60 is as good as infinity here and leaves the
-              // product finite
-              float q[16];
-#pragma unroll
-              for (int j = 32 * c; j < 32 * c + 32; ++j) x[j] = min_nan(x[j] * to_cap, 60.f);
-#pragma unroll
-              for (int j = 32 * c; j < 32 * c + 32; ++j) x[j] = ex2(x[j]);
-#pragma unroll
-              for (int j = 32 * c; j < 32 * c + 32; ++j) x[j] += 1.0f;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) q[j] = rcp(x[32 * c + 2 * j] * x[32 * c + 2 * j + 1]);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float d0 = x[32 * c + 2 * j], d1 = x[32 * c + 2 * j + 1];
-                q[j] *= -2.0f * cap2;
-                x[32 * c + 2 * j] = fmaf(q[j], d1, cap2);
-                x[32 * c + 2 * j + 1] = fmaf(q[j], d0, cap2);
-              }
-            } else {
-#pragma unroll
-              for (int j = 32 * c; j < 32 * c + 32; j += 2) unpair2(mul2(pair2(x[j], x[j + 1]), pair2(sl2, sl2)), x[j], x[j + 1]);
-            }
-            if (a.slopes) {
-              const float at = place_of_row - (float)((t - w.t0) * kTile);
-#pragma unroll
-              for (int j = 32 * c; j < 32 * c + 32; j += 2) {
-                const f32x2 far = pair2(fabsf(at - (float)j), fabsf(at - (float)(j + 1)));
-                unpair2(fma2(far, pair2(-slope2, -slope2), pair2(x[j], x[j + 1])), x[j], x[j + 1]);
-              }
-            }
-          }
-          if (masked) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[32 * c + j] = seen[c] & (1u << j) ? x[32 * c + j] : -INFINITY;
-          }
 #pragma unroll
           for (int j = 32 * c; j < 32 * c + 32; j += 4) {
             mx = max3(mx, x[j], x[j + 1]);
             mx1 = max3(mx1, x[j + 2], x[j + 3]);
           }
         }
-        mx = max_nan(mx, mx1);
-        if (!SCORE) mx *= sl2;
-        // a row moves by its own maximum alone: its result does not depend on the rows beside it; NaN moves it too
+        mx = max_nan(mx, mx1) * sl;
         if (i == 0) {
           m = mx;
         } else {
@@ -920,13 +958,13 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         const float base = m == -INFINITY ? 0.f : (m == INFINITY ? __int_as_float(0x7FC00000) : m);
         f32x2 sum = pair2(0.f, 0.f), sum1 = sum;
         auto probabilities = [&](int c) {      // exponentials and sum of 32 scores, and their probabilities into tensor memory
-          const f32x2 nb = pair2(-base, -base), sc = pair2(sl2, sl2);
+          const f32x2 nb = pair2(-base, -base), sc = pair2(sl, sl);
           uint32_t pk[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             const f32x2 xx = pair2(x[32 * c + 2 * j], x[32 * c + 2 * j + 1]);
             float e0, e1;
-            unpair2(SCORE ? add2(xx, nb) : fma2(xx, sc, nb), e0, e1);
+            unpair2(fma2(xx, sc, nb), e0, e1);
             e0 = ex2(e0);
             e1 = ex2(e1);
             if (j & 1) sum = add2(sum, pair2(e0, e1));
@@ -1207,8 +1245,7 @@ int make_head_map(CUtensorMap* map, const void* base, int64_t rows, int heads, i
 
 template <typename T, int DP>
 int launch_tc_t(const TileMaps& maps, const TcArgs& p, int grid, cudaStream_t s) {
-  const bool score = p.a.cap > 0.f || p.a.slopes;
-  const void* kern = score ? (const void*)masked_attention_kernel<T, DP, true> : (const void*)masked_attention_kernel<T, DP, false>;
+  const void* kern = (const void*)masked_attention_kernel<T, DP>;
   const size_t smem = (size_t)(2 + kRing) * kTile * DP * 2 + sizeof(Ctl);
   static_assert((2 + kRing) * kTile * DP * 2 + sizeof(Ctl) <= 227 * 1024, "shared memory of an SM");
   PMX_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
