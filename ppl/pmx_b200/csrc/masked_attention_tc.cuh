@@ -36,7 +36,7 @@ constexpr int kMaxSplits = 32;
 constexpr int kQueue = 4;                   // items under way
 constexpr int kMinTiles = 4;                // key tiles that a split of a pair of row tiles should have at least,
 constexpr int kFlatTiles = 2;               // and that a CTA should have of the list of all key tiles (2: one for each half;
-                                            // two drafted trees over 700 rows: 18.2 us against 20.7 us with 4)
+                                            // two drafted trees over 700 rows: a tenth faster than with 4)
 constexpr float kLazy = 8.0f;               // log2 of how far a maximum may run ahead
 constexpr unsigned long long kAttnWaitNs = 2000000000ull;
 
@@ -243,6 +243,13 @@ __device__ __forceinline__ f32x2 tanh_over_y(f32x2 y) {
   p = fma2(p, z, pair2(0x1.10e672p-3f, 0x1.10e672p-3f));
   p = fma2(p, z, pair2(-0x1.55540ap-2f, -0x1.55540ap-2f));
   return fma2(p, z, pair2(0x1.fffffep-1f, 0x1.fffffep-1f));
+}
+// the same in [-0.4, 0.4], degree 3: 9.8e-8, 1.5e-7 with the roundings
+__device__ __forceinline__ f32x2 tanh_over_y_near(f32x2 y) {
+  const f32x2 z = mul2(y, y);
+  f32x2 p = fma2(z, pair2(-0x1.858f22p-5f, -0x1.858f22p-5f), pair2(0x1.0fca24p-3f, 0x1.0fca24p-3f));
+  p = fma2(p, z, pair2(-0x1.55502ap-2f, -0x1.55502ap-2f));
+  return fma2(p, z, pair2(0x1.fffffcp-1f, 0x1.fffffcp-1f));
 }
 __device__ __forceinline__ float rcp(float x) {
   float y;
@@ -845,7 +852,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
     };
     // Cap, distance bias and mask: the scores of a tile as they have to be, written back to tensor memory.  A pass of its own
     // in a loop that is not unrolled, run only where there is something to do: the hot loop is as long as the instruction
-    // caches can bear (the same arithmetic inside it, unrolled, took 1184 us where this takes 961, and code that
+    // caches can bear (8192 capped tokens, otherwise alike: 961 us so, 1184 us with the same arithmetic unrolled in it; code that
     // was merely skipped cost a fifth).
     auto adjust = [&](const Work& w, int t, int whole, float slope2, float place_of_row) {
       uint32_t seen[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
@@ -871,8 +878,15 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
           float big = 0.f;
 #pragma unroll
           for (int j = 0; j < 32; j += 2) big = max3(big, fabsf(x[j]), fabsf(x[j + 1]));
-          if (__all_sync(0xFFFFFFFFu, big * to_y <= 1.0f)) {
-            // |s| <= c, as almost everywhere: tanh by its polynomial, off the special function unit
+          if (__all_sync(0xFFFFFFFFu, big * to_y <= 0.4f)) {
+            // |s| <= 0.4 c, as almost everywhere: the short polynomial (8192 capped tokens: 755 us, 835 us without it)
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const f32x2 xx = pair2(x[j], x[j + 1]);
+              unpair2(mul2(mul2(xx, pair2(sl2, sl2)), tanh_over_y_near(mul2(xx, pair2(to_y, to_y)))), x[j], x[j + 1]);
+            }
+          } else if (__all_sync(0xFFFFFFFFu, big * to_y <= 1.0f)) {
+            // tanh by its polynomial, off the special function unit
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               const f32x2 xx = pair2(x[j], x[j + 1]);
@@ -1171,33 +1185,52 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), t = row / a.Hq;
   if (t >= a.Tq) return;
-  int before = 0;
-  for (int i = lane; i <= a.B; i += 32) before += __ldcg(a.seqstarts + i) <= t ? 1 : 0;
+  // the row's sequence: the last that begins at or before it
+  int before = 0, start = 0;
+  for (int i = lane; i <= a.B; i += 32) {
+    const int64_t v = __ldcg(a.seqstarts + i);
+    if (v <= t) {
+      ++before;
+      start = v > start ? (int)v : start;
+    }
+  }
   const int b = __reduce_add_sync(0xFFFFFFFFu, before) - 1;
-  if (b < 0 || b >= a.B) return;
   const int head = (int)(row - t * a.Hq), h = head / p.group;
-  const int64_t i = t - clamp64(__ldcg(a.seqstarts + b), 0, a.Tq);
-  if (i < 0 || i >= a.max_seqlen) return;
+  const int64_t i = t - __reduce_max_sync(0xFFFFFFFFu, start);
+  if (b < 0 || b >= a.B || i >= a.max_seqlen) return;
   const int2 who = __ldcg(p.pieces + (int64_t)b * a.Hkv + h);
   if (who.x == who.y) return;                      // in one piece: the result is there
-  const int r = (int)i * p.group + head % p.group;
-  auto slot = [&](int c) { return c == who.x ? 2 * c + 1 : 2 * c; };
-  float top = -INFINITY;
-  for (int c = who.x + lane; c <= who.y; c += 32) top = fmaxf(top, __ldcg(p.part_ml + (int64_t)slot(c) * 128 + r).x);
+  const int r = (int)i * p.group + head % p.group, n = who.y - who.x + 1;
+  auto place = [&](int c) { return (int64_t)(c == 0 ? 2 * who.x + 1 : 2 * (who.x + c)) * 128 + r; };
+  auto stat = [&](int c) { return c < n ? __ldcg(p.part_ml + place(c)) : make_float2(-INFINITY, 0.f); };
+  auto values = [&](int c) {
+    return c < n && lane * 4 < a.D ? __ldcg(reinterpret_cast<const float4*>(p.part_o + place(c) * a.D) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+  };
+  // a lane has the maximum and sum of one piece; results are loaded four pieces ahead of what their factors wait for
+  float2 ml = stat(lane);
+  float4 v[4] = {values(0), values(1), values(2), values(3)};
+  float top = ml.x;
+  for (int c = 32; c < n; c += 32) top = fmaxf(top, stat(c + lane).x);
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c = who.x; c <= who.y; ++c) {
-    const float2 ml = __ldcg(p.part_ml + (int64_t)slot(c) * 128 + r);
-    if (ml.x == -INFINITY) continue;
-    const float f = ex2(ml.x - top);
-    sum = fmaf(ml.y, f, sum);
-    if (lane * 4 < a.D) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((int64_t)slot(c) * 128 + r) * a.D) + lane);
-      acc.x = fmaf(v.x, f, acc.x);
-      acc.y = fmaf(v.y, f, acc.y);
-      acc.z = fmaf(v.z, f, acc.z);
-      acc.w = fmaf(v.w, f, acc.w);
+  for (int c0 = 0; c0 < n; c0 += 4) {
+    if (c0 && (c0 & 31) == 0) ml = stat(c0 + lane);
+    const float f_lane = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int from = (c0 & 31) + k;
+      const float f = __shfl_sync(0xFFFFFFFFu, f_lane, from), l = __shfl_sync(0xFFFFFFFFu, ml.y, from);
+      const bool some = __shfl_sync(0xFFFFFFFFu, ml.x, from) != -INFINITY;
+      const float4 x = v[k];
+      v[k] = values(c0 + 4 + k);
+      if (some) {
+        sum = fmaf(l, f, sum);
+        acc.x = fmaf(x.x, f, acc.x);
+        acc.y = fmaf(x.y, f, acc.y);
+        acc.z = fmaf(x.z, f, acc.z);
+        acc.w = fmaf(x.w, f, acc.w);
+      }
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
