@@ -744,17 +744,21 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
     } else {
       // ---------------------------------------------------------------- cleaning, and drafted keys and values
       const int tid = threadIdx.x - 320;
-      {   // rows of no sequence: zeros, or partial results that count for nothing
-        const int64_t lo = clamp64(__ldcg(a.seqstarts), 0, a.Tq), hi = clamp64(__ldcg(a.seqstarts + a.B), lo, a.Tq);
-        const int64_t rows = (lo + a.Tq - hi) * a.Hq, step = (int64_t)gridDim.x * 2;
-        for (int64_t r = (int64_t)blockIdx.x * 2 + (tid >> 5); r < rows; r += step) {
-          const int64_t row = r < lo * a.Hq ? r : r + (hi - lo) * a.Hq;
+      {   // rows of no sequence, and those past max_seqlen: zeros, or partial results that count for nothing
+        auto blank = [&](int64_t row) {
           if (!p.pair || p.splits == 1) {
             T* out = reinterpret_cast<T*>(a.out) + row * a.D;
             for (int d = lane * 8; d < a.D; d += 256) *reinterpret_cast<uint4*>(out + d) = make_uint4(0, 0, 0, 0);
           } else if (lane < p.splits) {
             p.part_ml[(int64_t)lane * a.Tq * a.Hq + row] = make_float2(-INFINITY, 0.f);
           }
+        };
+        const int64_t lo = clamp64(__ldcg(a.seqstarts), 0, a.Tq), hi = clamp64(__ldcg(a.seqstarts + a.B), lo, a.Tq);
+        const int64_t rows = (lo + a.Tq - hi) * a.Hq, step = (int64_t)gridDim.x * 2;
+        for (int64_t r = (int64_t)blockIdx.x * 2 + (tid >> 5); r < rows; r += step) blank(r < lo * a.Hq ? r : r + (hi - lo) * a.Hq);
+        for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+          const int64_t first = clamp64(__ldcg(a.seqstarts + b), 0, a.Tq) + a.max_seqlen, end = clamp64(__ldcg(a.seqstarts + b + 1), 0, a.Tq);
+          for (int64_t r = first * a.Hq + (tid >> 5); r < end * a.Hq; r += 2) blank(r);
         }
       }
       uint32_t phases = 0, place_phase = 0;

@@ -19,8 +19,6 @@ from ._common import (cache_strides, exporting, heads, host, host_int, index, is
                       same_device, wants_grad)
 
 
-
-
 def _code(name: str, t: torch.Tensor) -> int:
     code = DTYPE_CODE.get(t.dtype)
     if code is None:
@@ -200,7 +198,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     scale * q.k (None: 1/sqrt(head_dim)), capped to logit_cap * tanh(score / logit_cap) where that is positive, less
     alibi_slopes[head] * |distance| where those are given.  A token that sees no key, and a row of no sequence, is zero;
     what a token may not see does not reach its result, whatever it holds.
-    max_seqlen, max_kvlen (int or one-element tensor): at least the longest sequence's queries and keys.
+    max_seqlen, max_kvlen (int or one-element tensor): at least the longest sequence's queries and keys.  The rows
+    of a sequence behind its first max_seqlen are zero.
     query, key and value may be views with unit inner stride.  float16, bfloat16, float32, head_dim up to 256."""
     args = (query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_heads, head_dim, is_causal, num_kv_heads,
             scale, float(logit_cap), alibi_slopes, prefix_lens)

@@ -192,6 +192,44 @@ def test_prompt_attention_groups(DB, Hq, Hkv):
     run_prompt(DB, "f16", [(19, 60), (3, 3)], Hq, Hkv, 64)
 
 
+@pytest.mark.parametrize("dtype,Hq,Hkv,D,causal,alibi", [("bf16", 4, 2, 64, True, False), ("f16", 3, 3, 128, True, True),
+                                                         ("bf16", 2, 1, 80, False, False)])
+def test_prompt_attention_of_many_ragged_sequences(DB, dtype, Hq, Hkv, D, causal, alibi):
+    """More sequences than a warp has lanes, empty ones among them, several rounds of items for every CTA."""
+    rng = np.random.default_rng(21)
+    lens = [(int(n), int(n + more)) for n, more in zip(rng.integers(0, 280, 75), rng.integers(0, 3, 75) * 50)]
+    lens[0], lens[40], lens[74] = (0, 0), (0, 17), (300, 300)
+    run_prompt(DB, dtype, lens, Hq, Hkv, D, causal=causal, alibi=alibi, extra=2)
+
+
+@pytest.mark.parametrize("rows,Hq,Hkv,D", [(4, 2, 1, 128), (1, 1, 1, 64), (9, 6, 2, 40)])
+def test_few_rows_over_keys_in_many_pieces(DB, rows, Hq, Hkv, D):
+    """A long key axis is cut into more pieces than a warp has lanes, next to sequences of one piece and of none."""
+    run_prompt(DB, "bf16", [(3, 60), (rows, 9100), (0, 5), (2, 2)], Hq, Hkv, D)
+
+
+@pytest.mark.parametrize("cap", [0.5, 2.0, 4.0, 12.0])
+def test_scores_around_the_cap(DB, cap):
+    """Scores from far below the cap to far above it: tanh by either polynomial and by the exponential, in all mixtures."""
+    run_prompt(DB, "f16", [(130, 130), (7, 300)], 2, 1, 64, cap=cap, scale=0.2)
+
+
+@pytest.mark.parametrize("lens,most", [([(20, 20), (7, 30)], 9), ([(300, 300), (90, 200)], 150), ([(3, 2000)], 2),
+                                       ([(200, 3000)], 150)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_past_max_seqlen_are_zero(DB, dtype, lens, most):
+    rng = np.random.default_rng(2)
+    q, k, v, ss, ks, _, mk = prompt_case(rng, lens, 2, 1, 64, dtype)
+    args = (dev(q, dtype), dev(k, dtype), dev(v, dtype), i64(ss), i64(ks))
+    torch.full((1 << 20,), float("nan"), device="cuda")               # freed: what the results' memory may hold
+    got = DB.prompt_attention(*args, most, mk, 2, 64, num_kv_heads=1)
+    o, A, dots, tops = ab.prompt_attention(q, k, v, ss, ks, True, 1 / 8.0, 0.0, None, None)
+    keep = np.concatenate([np.arange(s, min(s + most, e)) for s, e in zip(ss[:-1], ss[1:])])
+    rest = np.setdiff1d(np.arange(len(q)), keep)
+    check_attention(got[torch.from_numpy(keep).cuda()], (o[keep], A[keep], dots[keep], tops[keep]), dtype, 64, mk, 0.0)
+    assert len(rest) and not got[torch.from_numpy(rest).cuda()].any()
+
+
 @pytest.mark.parametrize("lens", [[(300, 300)], [(2, 1500)], [(600, 600), (1, 700)]])
 def test_rows_of_no_sequence_are_zero(DB, lens):
     got, ss = run_prompt(DB, "bf16", lens, 4, 2, 128, extra=5)
