@@ -226,7 +226,7 @@ PyObject* prompt(PyObject* const* args, Py_ssize_t n) {
   a.logit_cap = c.real(12);
   a.dtype = dtype_code(type);
   if (!c.ready() || a.dtype < 0 || a.max_seqlen <= 0 || a.max_kvlen <= 0 || (args[9] != Py_True && args[9] != Py_False) ||
-      (prefix && !a.is_causal) || !(a.scale > 0.0) || std::isinf(a.scale) || !(a.logit_cap >= 0.0) || std::isinf(a.logit_cap) ||
+      !(a.scale > 0.0) || std::isinf(a.scale) || !(a.logit_cap >= 0.0) || std::isinf(a.logit_cap) ||
       a.num_heads % a.num_kv_heads ||
       (slopes && (slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != a.num_heads || !slopes->is_contiguous())))
     return none();

@@ -72,8 +72,6 @@ def _prompt(query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_h
         raise ValueError(f"{name}: `seqstarts` must hold the start of every sequence and the end")
     seqstarts, kvstarts = index(name, "seqstarts", seqstarts, B + 1), index(name, "kvstarts", kvstarts, B + 1)
     if prefix_lens is not None:
-        if not is_causal:
-            raise ValueError(f"{name}: prefix_lens go with is_causal (without it every token sees its whole sequence)")
         prefix_lens = index(name, "prefix_lens", prefix_lens, B)
     if alibi_slopes is not None:
         if tuple(alibi_slopes.shape) != (num_heads,):
@@ -194,9 +192,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     Sequence b holds the queries seqstarts[b]..seqstarts[b+1] and the keys kvstarts[b]..kvstarts[b+1]; its queries are the
     last of its positions (a chunk of a prompt behind what is there already).  No token sees another sequence: starts at
     document borders are a document mask.  is_causal: a token sees the positions up to its own, and with
-    `prefix_lens` [B] all of the first prefix_lens[b] as well; otherwise its whole sequence.  Scores are
-    scale * q.k (None: 1/sqrt(head_dim)), capped to logit_cap * tanh(score / logit_cap) where that is positive, less
-    alibi_slopes[head] * |distance| where those are given.  A token that sees no key, and a row of no sequence, is zero;
+    `prefix_lens` [B] all of the first prefix_lens[b] as well; otherwise its whole sequence, to which a prefix adds
+    nothing.  Scores are scale * q.k (None: 1/sqrt(head_dim)), capped to logit_cap * tanh(score / logit_cap) where that is
+    positive, less alibi_slopes[head] * |distance| where those are given.  A token that sees no key, and a row of no sequence, is zero;
     what a token may not see does not reach its result, whatever it holds.
     max_seqlen, max_kvlen (int or one-element tensor): at least the longest sequence's queries and keys.  The rows
     of a sequence behind its first max_seqlen are zero.

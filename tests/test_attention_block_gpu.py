@@ -181,7 +181,7 @@ def test_prompt_attention_lengths_and_heads(DB, lens, dtype, Hq, Hkv, D):
 
 @pytest.mark.parametrize("options", [dict(causal=False), dict(cap=5.0), dict(alibi=True), dict(prefix=[20, 0, 300, 7]),
                                      dict(cap=30.0, alibi=True, prefix=[100, 1, 0, 40]), dict(scale=0.01), dict(scale=3.0),
-                                     dict(causal=False, alibi=True)])
+                                     dict(causal=False, alibi=True), dict(causal=False, cap=9.0, prefix=[20, 0, 300, 7])])
 @pytest.mark.parametrize("dtype,Hq,Hkv,D", [("bf16", 8, 2, 128), ("f16", 2, 2, 64), ("f32", 2, 1, 32)])
 def test_prompt_attention_options(DB, options, dtype, Hq, Hkv, D):
     run_prompt(DB, dtype, [(140, 140), (1, 9), (30, 350), (40, 40)], Hq, Hkv, D, **options)
@@ -331,7 +331,7 @@ def test_prompt_attention_refuses(DB):
                          (dict(max_seqlen=0), ValueError), (dict(max_kvlen=-1), ValueError), (dict(scale=0.0), ValueError),
                          (dict(scale=float("nan")), ValueError), (dict(logit_cap=-2.0), ValueError),
                          (dict(alibi_slopes=torch.ones(3, device="cuda")), ValueError), (dict(prefix_lens=i64([1, 2])), ValueError),
-                         (dict(prefix_lens=i64([3]), is_causal=False), ValueError), (dict(kvstarts=ss.cpu()), RuntimeError),
+                         (dict(kvstarts=ss.cpu()), RuntimeError),
                          (dict(query=q.double(), key=k.double(), value=k.double()), TypeError), (dict(query=q.view(24, 64)), ValueError)):
         with pytest.raises(kind):
             DB.prompt_attention(**{**ok, **change})
