@@ -12,7 +12,7 @@
 //            O_w += P_w V into columns [256 + 128 w, +128); P_w is read from tensor memory, V is the MN-major operand
 //   warps 0-3 and 4-7  the softmax of S_0 and S_1, one thread per row (a thread owns a tensor memory lane, so the
 //            row's maximum and sum need no exchange); P_w overwrites S_w in 16 bits and is handed over in two halves
-//   warps 10, 11  go over those value tiles of which some rows see a part only, and store drafted keys and values
+//   warps 10, 11  store drafted keys and values, then go over those value tiles of which some rows see a part only
 // With more than 128 rows (`pair`) the two tiles share the keys; an item is one block of rows, the longest first.  With
 // fewer, both softmax halves work on the same rows, on the even and the odd key tiles, and meet at the end; the
 // key tiles of all (sequence, key head) pairs are then dealt out evenly over the CTAs as one long list, and what a cut
@@ -56,6 +56,7 @@ struct TcArgs {
   int2* pieces;
   int group, tokens;                        // query heads per key head, tokens of a row tile
   int row_blocks, splits, pair;
+  int ctas;                                 // CTAs that the workspace has room for; more may run, with nothing but stores to do
   int flat;                                 // not pair: cut the list of key tiles evenly (otherwise whole items)
 };
 
@@ -67,7 +68,6 @@ struct Work {
   int t0, nt[2];       // first key tile; tiles of each row tile (without pair: nt[0] is the item's)
   int drafted;         // index of the drafted tokens' tile, -1: none
   int partial;         // first tile that some row does not see whole
-  int stores;          // this item stores the sequence's drafted keys and values of this head
   int number;          // of the item in this CTA, from 1
 };
 
@@ -309,7 +309,6 @@ __device__ __forceinline__ void finish_work(const TcArgs& p, Work& w, int t0, in
   w.nt[0] = (n0 < t1 ? n0 : t1) - w.t0;
   if (w.nt[0] < 0) w.nt[0] = 0;
   w.nt[1] = w.halves == 2 ? t1 - w.t0 : 0;
-  w.stores = a.tree_mask && w.tok0 == 0 && t0 == 0;
 }
 
 // The items of one CTA, in order.  Run by all lanes of a warp.
@@ -350,7 +349,7 @@ struct Items {
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     total = sum * a.Hkv;
     const int64_t most = total / kFlatTiles;
-    ctas = (int)(most < 1 ? 1 : (most < (int64_t)gridDim.x ? most : (int64_t)gridDim.x));
+    ctas = (int)(most < 1 ? 1 : (most < p.ctas ? most : p.ctas));
     u = (int)blockIdx.x < ctas ? (int64_t)blockIdx.x * total / ctas : total;
     u1 = (int)blockIdx.x < ctas ? (int64_t)(blockIdx.x + 1) * total / ctas : total;
     if (u >= u1) return;
@@ -761,6 +760,51 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
           for (int64_t r = first * a.Hq + (tid >> 5); r < end * a.Hq; r += 2) blank(r);
         }
       }
+      if (a.tree_mask) {
+        // Drafted keys and values into the cache, where this launch does not read them: a run of tokens for each of these
+        // warps of the whole grid.  (Stored by the CTAs that read them, the rows of one head by one CTA, a single tree of
+        // 62 tokens took 25 us; so it takes 14.)
+        const int64_t warps = (int64_t)gridDim.x * 2, run = (a.Tq + warps - 1) / warps;
+        const int64_t ta = ((int64_t)blockIdx.x * 2 + (tid >> 5)) * run, tb = ta + run < a.Tq ? ta + run : a.Tq;
+        const int chunks = a.D / 8, count = a.Hkv * 2 * chunks;
+        int64_t end = ta;                             // the first token that needs a look-up
+        Sequence s;
+        s.n = 0;
+        s.q0 = s.kv0 = s.len = 0;
+        for (int64_t t = ta; t < tb; ++t) {
+          if (t >= end) {
+            int before = 0;
+            for (int i = lane; i <= a.B; i += 32) before += __ldcg(a.seqstarts + i) <= t ? 1 : 0;
+            const int b = __reduce_add_sync(0xFFFFFFFFu, before) - 1;
+            end = t + 1;
+            s.n = 0;
+            if (b >= 0 && b < a.B) {
+              s = load_sequence(a, b);
+              if (t < s.q0 + s.n) end = s.q0 + s.n;
+            }
+          }
+          const int64_t row = s.kv0 + s.len + (t - s.q0);
+          if (t - s.q0 < 0 || t - s.q0 >= s.n || row >= a.past.rows) continue;
+          for (int i0 = lane; i0 < count; i0 += 32 * 4) {
+            uint4 held[4];
+            T* dst[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int i = i0 + 32 * j, hk = i / chunks, ch = i - hk * chunks, h = hk >> 1;
+              dst[j] = nullptr;
+              if (i < count) {
+                held[j] = ld_stream16(hk & 1 ? reinterpret_cast<const T*>(a.cur.v) + t * a.cur.v_row + h * a.cur.v_head + ch * 8
+                                             : reinterpret_cast<const T*>(a.cur.k) + t * a.cur.k_row + h * a.cur.k_head + ch * 8);
+                dst[j] = (hk & 1 ? reinterpret_cast<T*>(const_cast<void*>(a.past.v)) + row * a.past.v_row + h * a.past.v_head
+                                 : reinterpret_cast<T*>(const_cast<void*>(a.past.k)) + row * a.past.k_row + h * a.past.k_head) + ch * 8;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (dst[j]) *reinterpret_cast<uint4*>(dst[j]) = held[j];
+          }
+        }
+      }
       uint32_t phases = 0, place_phase = 0;
       int place = 0, entry0 = 0;
       bool ok = true;
@@ -771,19 +815,6 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         const Work& w = ctl->work[place];
         if (w.h < 0) break;
         const int total = tiles_of(w);
-        if (w.stores) {
-          // into the cache, where this launch does not read them
-          for (int i = tid; i < w.s.n * (a.D / 8) * 2; i += 64) {
-            const int ch = i % (a.D / 8), kv = i / (a.D / 8) & 1, t = i / (a.D / 8) >> 1;
-            const int64_t row = w.s.kv0 + w.s.len + t;
-            if (row >= a.past.rows) continue;
-            const T* src = kv ? reinterpret_cast<const T*>(a.cur.v) + (w.s.q0 + t) * a.cur.v_row + w.h * a.cur.v_head
-                              : reinterpret_cast<const T*>(a.cur.k) + (w.s.q0 + t) * a.cur.k_row + w.h * a.cur.k_head;
-            T* dst = kv ? reinterpret_cast<T*>(const_cast<void*>(a.past.v)) + row * a.past.v_row + w.h * a.past.v_head
-                        : reinterpret_cast<T*>(const_cast<void*>(a.past.k)) + row * a.past.k_row + w.h * a.past.k_head;
-            *reinterpret_cast<uint4*>(dst + ch * 8) = ld_stream16(src + ch * 8);
-          }
-        }
         for (int i = w.partial > w.t0 ? w.partial - w.t0 : 0; i < total && ok; ++i) {
           const int entry = 2 * i + lag < total + i ? 2 * i + lag : total + i;     // of the values of tile i
           const int slot = (entry0 + entry) % kRing;
@@ -1349,6 +1380,9 @@ int launch_tc(const AttnArgs& a, const TcPlan& pl, int dtype, const char* name, 
   p.a = a;
   p.group = pl.group; p.tokens = pl.tokens; p.row_blocks = pl.row_blocks; p.splits = pl.splits; p.pair = pl.pair;
   p.flat = pl.flat;
+  p.ctas = pl.grid;
+  int64_t grid = pl.grid;
+  if (a.tree_mask && grid < ceil_div(a.Tq, 2)) grid = ceil_div(a.Tq, 2) < sm_count() ? ceil_div(a.Tq, 2) : sm_count();
   size_t o_at = 0, pieces_at = 0;
   tc_workspace(pl, a.Tq, a.B, a.Hq, a.Hkv, a.D, &o_at, &pieces_at);
   p.part_ml = reinterpret_cast<float2*>(ws);
@@ -1362,6 +1396,6 @@ int launch_tc(const AttnArgs& a, const TcPlan& pl, int dtype, const char* name, 
   if (st == PMX_OK && a.tree_mask) st = make_head_map(&m.cv, a.cur.v, a.cur.rows, a.Hkv, a.D, a.cur.v_row, a.cur.v_head, 1, kTreeLimit, dtype, name);
   if (st != PMX_OK) return st;
   const bool bf = dtype == PMX_DTYPE_BF16;
-  if (a.D <= 64) return bf ? launch_tc_t<__nv_bfloat16, 64>(m, p, pl.grid, s) : launch_tc_t<__half, 64>(m, p, pl.grid, s);
-  return bf ? launch_tc_t<__nv_bfloat16, 128>(m, p, pl.grid, s) : launch_tc_t<__half, 128>(m, p, pl.grid, s);
+  if (a.D <= 64) return bf ? launch_tc_t<__nv_bfloat16, 64>(m, p, (int)grid, s) : launch_tc_t<__half, 64>(m, p, (int)grid, s);
+  return bf ? launch_tc_t<__nv_bfloat16, 128>(m, p, (int)grid, s) : launch_tc_t<__half, 128>(m, p, (int)grid, s);
 }
