@@ -56,6 +56,7 @@ struct TcArgs {
   int2* pieces;
   int group, tokens;                        // query heads per key head, tokens of a row tile
   int row_blocks, splits, pair;
+  int pieces_of_item;                       // about the most, from the host's lengths
   int ctas;                                 // CTAs that the workspace has room for; more may run, with nothing but stores to do
   int flat;                                 // not pair: cut the list of key tiles evenly (otherwise whole items)
 };
@@ -1211,14 +1212,19 @@ __global__ void __launch_bounds__(256) masked_attention_merge_kernel(const float
   }
 }
 
-// The same for items whose key tiles were dealt out: one warp per row, the pieces of its item.
-template <typename T>
+// The same for items whose key tiles were dealt out: WARPS warps per row share the pieces of its item.  One warp up to
+// four pieces, whose loads are all under way at once; beyond, a block, as a single warp would wait for memory once for every
+// four (one row over 100 000 keys, 148 pieces: 30 us, 48 us with one warp; eight drafted tokens over 12 000: 18 and 27).
+template <typename T, int WARPS>
 __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid_constant__ TcArgs p) {
+  __shared__ float4 shares[WARPS > 1 ? 8 : 1][32];
+  __shared__ float sums[8];
   pdl_launch_dependents();
   pdl_wait();
   const AttnArgs& a = p.a;
   const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), t = row / a.Hq;
+  const int warp = threadIdx.x >> 5, part = warp % WARPS;
+  const int64_t row = ((int64_t)blockIdx.x * 8 + warp) / WARPS, t = row / a.Hq;
   if (t >= a.Tq) return;
   // the row's sequence: the last that begins at or before it
   int before = 0, start = 0;
@@ -1235,22 +1241,23 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
   if (b < 0 || b >= a.B || i >= a.max_seqlen) return;
   const int2 who = __ldcg(p.pieces + (int64_t)b * a.Hkv + h);
   if (who.x == who.y) return;                      // in one piece: the result is there
-  const int r = (int)i * p.group + head % p.group, n = who.y - who.x + 1;
+  const int r = (int)i * p.group + head % p.group, n = who.y - who.x + 1;         // pieces, of which this warp takes every WARPS-th
   auto place = [&](int c) { return (int64_t)(c == 0 ? 2 * who.x + 1 : 2 * (who.x + c)) * 128 + r; };
   auto stat = [&](int c) { return c < n ? __ldcg(p.part_ml + place(c)) : make_float2(-INFINITY, 0.f); };
   auto values = [&](int c) {
     return c < n && lane * 4 < a.D ? __ldcg(reinterpret_cast<const float4*>(p.part_o + place(c) * a.D) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
   };
-  // a lane has the maximum and sum of one piece; results are loaded four pieces ahead of what their factors wait for
-  float2 ml = stat(lane);
-  float4 v[4] = {values(0), values(1), values(2), values(3)};
+  // a lane has the maximum and sum of one of the warp's pieces; results are loaded four pieces ahead of what their factors
+  // wait for
+  float2 ml = stat(part + lane * WARPS);
+  float4 v[4] = {values(part), values(part + WARPS), values(part + 2 * WARPS), values(part + 3 * WARPS)};
   float top = ml.x;
-  for (int c = 32; c < n; c += 32) top = fmaxf(top, stat(c + lane).x);
+  for (int c = WARPS > 1 ? lane : lane + 32; c < n; c += 32) top = fmaxf(top, stat(c).x);
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   float sum = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int c0 = 0; c0 < n; c0 += 4) {
-    if (c0 && (c0 & 31) == 0) ml = stat(c0 + lane);
+  for (int c0 = 0; part + c0 * WARPS < n; c0 += 4) {
+    if (c0 && (c0 & 31) == 0) ml = stat(part + (c0 + lane) * WARPS);
     const float f_lane = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -1258,7 +1265,7 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
       const float f = __shfl_sync(0xFFFFFFFFu, f_lane, from), l = __shfl_sync(0xFFFFFFFFu, ml.y, from);
       const bool some = __shfl_sync(0xFFFFFFFFu, ml.x, from) != -INFINITY;
       const float4 x = v[k];
-      v[k] = values(c0 + 4 + k);
+      v[k] = values(part + (c0 + 4 + k) * WARPS);
       if (some) {
         sum = fmaf(l, f, sum);
         acc.x = fmaf(x.x, f, acc.x);
@@ -1266,6 +1273,20 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
         acc.z = fmaf(x.z, f, acc.z);
         acc.w = fmaf(x.w, f, acc.w);
       }
+    }
+  }
+  if (WARPS > 1) {
+    shares[warp][lane] = acc;
+    sums[warp] = sum;
+    __syncthreads();                // all warps of the block have the same row, none has left
+    if (part) return;
+    for (int o = 1; o < WARPS; ++o) {
+      const float4 x = shares[o][lane];
+      acc.x += x.x;
+      acc.y += x.y;
+      acc.z += x.z;
+      acc.w += x.w;
+      sum += sums[o];
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
@@ -1280,7 +1301,7 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
 // ------------------------------------------------------------------------------------------------- host side
 struct TcPlan {
   bool use;
-  int group, tokens, pair, row_blocks, splits, flat, grid;
+  int group, tokens, pair, row_blocks, splits, flat, grid, pieces;
 };
 
 // Everything that sizes the workspace and the grid follows from shapes and host lengths alone.
@@ -1313,6 +1334,8 @@ TcPlan plan_tc(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_
     grid = pl.flat ? ceil_div(items * tiles, kFlatTiles) : items;
   }
   pl.grid = (int)(grid < sms ? grid : sms);
+  const int64_t each = ceil_div(items * tiles, pl.grid);           // key tiles of a CTA
+  pl.pieces = (int)ceil_div(tiles, each < kFlatTiles ? kFlatTiles : each);
   pl.use = true;
   return pl;
 }
@@ -1360,7 +1383,9 @@ int launch_tc_t(const TileMaps& maps, const TcArgs& p, int grid, cudaStream_t s)
   if (st != PMX_OK || (p.splits == 1 && !p.flat)) return st;
   const int64_t rows = p.a.Tq * p.a.Hq;
   const dim3 merge_grid((unsigned)ceil_div(rows, 8)), merge_block(256);
-  if (p.flat) return launch_pdl_k(masked_attention_join_kernel<T>, merge_grid, merge_block, 0, s, p);
+  if (p.flat && p.pieces_of_item > 4 && p.a.Tq * p.a.Hq < (1ll << 31))      // a block per row
+    return launch_pdl_k(masked_attention_join_kernel<T, 8>, dim3((unsigned)(p.a.Tq * p.a.Hq)), merge_block, 0, s, p);
+  if (p.flat) return launch_pdl_k(masked_attention_join_kernel<T, 1>, merge_grid, merge_block, 0, s, p);
   return launch_pdl_k(masked_attention_merge_kernel<T>, merge_grid, merge_block, 0, s, (const float*)p.part_o,
                       (const float2*)p.part_ml, (T*)p.a.out, rows, p.a.D, p.splits);
 }
@@ -1381,6 +1406,7 @@ int launch_tc(const AttnArgs& a, const TcPlan& pl, int dtype, const char* name, 
   p.group = pl.group; p.tokens = pl.tokens; p.row_blocks = pl.row_blocks; p.splits = pl.splits; p.pair = pl.pair;
   p.flat = pl.flat;
   p.ctas = pl.grid;
+  p.pieces_of_item = pl.pieces;
   int64_t grid = pl.grid;
   if (a.tree_mask && grid < ceil_div(a.Tq, 2)) grid = ceil_div(a.Tq, 2) < sm_count() ? ceil_div(a.Tq, 2) : sm_count();
   size_t o_at = 0, pieces_at = 0;
