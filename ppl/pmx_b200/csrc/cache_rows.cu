@@ -3,12 +3,12 @@
 // Sequence b has stored drafted tokens at rows base, base + 1, ... with base = cachestarts[b] +
 // start_pos[b]; the accepted ones, accept_index[accept_starts[b] ..], move to the front:
 // row base + i <- row base + accept_index[i], in all layers, keys and values, all reads before all
-// writes.  Bound by the bytes of the rows that move.  A block looks the rows of its sequence up once and then walks
-// over columns (the same 16 bytes of every row): a thread has one to four rows and eight of its row's or rows'
-// vectors under way, and the block holds all rows of the columns at hand between its reads and its writes, which a
-// barrier keeps apart: any indices (repeated, descending) are right.  For 32 sequences of up to 19 rows of 128 KB,
-// out of HBM: 31 us; one thread per column with all its rows 50 us (few warps), one vector per thread
-// and block 79 us (the look-up's three memory latencies in every block).
+// writes.  Bound by the bytes of the rows that move.  A block looks the rows of its sequence up once; its warps then walk
+// over columns (the same 16 bytes of every row), and a warp holds all rows of the columns at hand between its reads and its
+// writes, eight or sixteen vectors a lane: any indices (repeated, descending) are right, and no warp waits for another.  For
+// 32 sequences in 32 layers, out of HBM: 24 us with up to 19 rows of 128 KB, 9.6 us with up to 10; whole blocks that
+// read, meet at a barrier and write took 30 and 21 us, one thread per column with all its rows 50 (few warps), one
+// vector per thread and block 79 (the look-up's three memory latencies in every block).
 #include "common.cuh"
 
 namespace pmx {
@@ -22,67 +22,88 @@ struct CompactArgs {
   int layers, heads, chunks;                              // chunks: vectors of a head row
 };
 
-constexpr int kThreads = 256, kVectors = 8;      // vectors that a thread has under way
+constexpr int kWarps = 8;
+constexpr int kMaxAccept = 64;
 
-// `slots` rows (a power of two) times 256 / slots columns at a time, ROWS rows per thread
-template <typename VEC, int ROWS>
-__global__ void __launch_bounds__(kThreads) compact_cache_kernel(const CompactArgs a, int slots, int slot_bits) {
-  constexpr int GROUPS = kVectors / ROWS;
+// W columns side by side, 32 / W rows to a step; a lane has kVectors vectors under way
+template <typename VEC, int W, int kVectors>
+__global__ void __launch_bounds__(kWarps * 32) compact_cache_kernel(const __grid_constant__ CompactArgs a) {
+  constexpr int R = 32 / W;
+  __shared__ int64_t moves[2][kMaxAccept];       // byte offsets from and to which rows move
+  __shared__ int count;
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.y;
-  const int64_t first = __ldcg(a.accept_starts + b), last = __ldcg(a.accept_starts + b + 1);
-  const int64_t base = __ldcg(a.cachestarts + b) + __ldcg(a.start_pos + b);
-  if (first < 0 || last > a.index_count) return;
-  const int n = (int)(last - first < ROWS * slots ? last - first : ROWS * slots);
-  const int cols = kThreads >> slot_bits, row = threadIdx.x / cols;
-  int64_t src[ROWS], dst[ROWS];                  // byte offsets of this thread's rows
-  bool moves[ROWS];
-#pragma unroll
-  for (int k = 0; k < ROWS; ++k) {
-    const int i = row + k * slots;
-    const int64_t from = i < n ? __ldcg(a.accept_index + first + i) : -1;
-    // a row that stays, or one outside the cache, is left alone
-    moves[k] = from >= 0 && from != i && base + from >= 0 && base + from < a.rows && base + i >= 0 && base + i < a.rows;
-    src[k] = (base + from) * a.row_bytes;
-    dst[k] = (base + i) * a.row_bytes;
-  }
-  const uint32_t columns = (uint32_t)a.layers * 2 * a.heads * a.chunks, step = gridDim.x * cols;      // below 2^30
-  for (uint32_t c0 = blockIdx.x * cols; c0 < columns; c0 += GROUPS * step) {
-    VEC held[GROUPS][ROWS];
-    char* at[GROUPS];
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      const uint32_t col = c0 + g * step + (threadIdx.x - row * cols);
-      const uint32_t hh = col / (uint32_t)a.chunks, ch = col - hh * a.chunks, lk = hh / (uint32_t)a.heads, h = hh - lk * a.heads;
-      at[g] = col < columns ? a.cache + (int64_t)(lk >> 1) * a.layer_bytes + (int64_t)(lk & 1) * a.kv_bytes + (int64_t)h * a.head_bytes + (int64_t)(ch * sizeof(VEC)) : nullptr;
-#pragma unroll
-      for (int k = 0; k < ROWS; ++k)
-        if (at[g] && moves[k]) held[g][k] = __ldcg(reinterpret_cast<const VEC*>(at[g] + src[k]));
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp == 0) {
+    const int64_t first = __ldcg(a.accept_starts + b), last = __ldcg(a.accept_starts + b + 1);
+    const int64_t base = __ldcg(a.cachestarts + b) + __ldcg(a.start_pos + b);
+    const int64_t n = first < 0 || last > a.index_count ? 0 : (last - first < R * kVectors ? last - first : R * kVectors);
+    int before = 0;
+    for (int i = lane; i < kMaxAccept; i += 32) {
+      const int64_t from = i < n ? __ldcg(a.accept_index + first + i) : -1;
+      // a row that stays, or one outside the cache, is left alone
+      const bool on = from >= 0 && from != i && base + from >= 0 && base + from < a.rows && base + i >= 0 && base + i < a.rows;
+      const unsigned some = __ballot_sync(0xFFFFFFFFu, on);
+      if (on) {
+        const int at = before + __popc(some & ((1u << lane) - 1));
+        moves[0][at] = (base + from) * a.row_bytes;
+        moves[1][at] = (base + i) * a.row_bytes;
+      }
+      before += __popc(some);
     }
-    __syncthreads();
+    if (lane == 0) count = before;
+  }
+  __syncthreads();
+  const int m = count, steps = (m + R - 1) / R, row = lane / W;
+  if (m == 0) return;
+  const uint32_t columns = (uint32_t)a.layers * 2 * a.heads * a.chunks;              // below 2^30
+  const uint32_t units = (columns + W - 1) / W, stride = gridDim.x * kWarps;
+  uint32_t unit = blockIdx.x * kWarps + warp;
+  while (unit < units) {
+    VEC held[kVectors];
+    char* to[kVectors];
+    char* at = nullptr;
+    int step = steps;
+    const uint32_t full = kVectors / steps;      // units of this round
+    uint32_t next = unit;
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g)
+    for (int k = 0; k < kVectors; ++k) {
+      to[k] = nullptr;
+      if (step == steps) {
+        step = 0;
+        const uint32_t col = next * W + (lane & (W - 1));
+        const uint32_t hh = col / (uint32_t)a.chunks, ch = col - hh * a.chunks, lk = hh / (uint32_t)a.heads, h = hh - lk * a.heads;
+        at = next < unit + full * stride && col < columns && next < units
+                 ? a.cache + (int64_t)(lk >> 1) * a.layer_bytes + (int64_t)(lk & 1) * a.kv_bytes + (int64_t)h * a.head_bytes + (int64_t)(ch * sizeof(VEC))
+                 : nullptr;
+        next += stride;
+      }
+      const int i = step * R + row;
+      if (at && i < m) {
+        held[k] = __ldcg(reinterpret_cast<const VEC*>(at + moves[0][i]));
+        to[k] = at + moves[1][i];
+      }
+      ++step;
+    }
+    __syncwarp();                                // all reads of the columns at hand before the writes
 #pragma unroll
-      for (int k = 0; k < ROWS; ++k)
-        if (at[g] && moves[k]) *reinterpret_cast<VEC*>(at[g] + dst[k]) = held[g][k];
+    for (int k = 0; k < kVectors; ++k)
+      if (to[k]) *reinterpret_cast<VEC*>(to[k]) = held[k];
+    unit += full * stride;
   }
 }
 
 template <typename VEC>
 int launch_compact_vec(const CompactArgs& a, int max_accept, int64_t B, cudaStream_t s) {
-  // a row per thread up to 16 accepted rows (16 columns of 16 bytes: a block still touches whole 256-byte head rows), then two
-  // or four
-  int bits = 0;
-  while (bits < 4 && (1 << bits) < max_accept) ++bits;
-  const int slots = 1 << bits;
-  const int64_t groups = ceil_div((int64_t)a.layers * 2 * a.heads * a.chunks, kThreads / slots);
-  // as many blocks as are resident at once, each with at least one round of loads
-  const int64_t most = ceil_div((int64_t)sm_count() * 6, B), rounds = ceil_div(groups, max_accept <= 16 ? 8 : max_accept <= 32 ? 4 : 2);
-  const dim3 grid((unsigned)(rounds < most ? rounds : most), (unsigned)B), block(kThreads);
-  if (max_accept <= 16) return launch_pdl_k(compact_cache_kernel<VEC, 1>, grid, block, 0, s, a, slots, bits);
-  if (max_accept <= 32) return launch_pdl_k(compact_cache_kernel<VEC, 2>, grid, block, 0, s, a, slots, bits);
-  return launch_pdl_k(compact_cache_kernel<VEC, 4>, grid, block, 0, s, a, slots, bits);
+  // 16 columns side by side are the 256 bytes of a usual head's row; more rows than 16 take twice the registers, more
+  // than 32 half the columns.  Up to eight blocks per SM: 26 and 27 us in the case above with twelve and sixteen.
+  const int w = max_accept <= 32 ? 16 : 8;
+  const int64_t blocks = ceil_div(ceil_div((int64_t)a.layers * 2 * a.heads * a.chunks, w), kWarps);
+  const int64_t most = ceil_div((int64_t)sm_count() * 8, B);
+  const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)B), block(kWarps * 32);
+  if (max_accept <= 16) return launch_pdl_k(compact_cache_kernel<VEC, 16, 8>, grid, block, 0, s, a);
+  if (max_accept <= 32) return launch_pdl_k(compact_cache_kernel<VEC, 16, 16>, grid, block, 0, s, a);
+  return launch_pdl_k(compact_cache_kernel<VEC, 8, 16>, grid, block, 0, s, a);
 }
 
 }  // namespace
