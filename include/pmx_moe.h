@@ -411,7 +411,8 @@ int pmx_rotary_embedding(const pmx_rotary_args* args, void* stream);
  *   out = softmax(s) v over the keys seen; a query that sees none, and a row of no sequence, is zero.
  * What a query may not see does not reach its result, whatever it holds (infinities and NaN included).
  * seqstarts, kvstarts [B+1], prefix_lens [B] int64 on the device; max_seqlen / max_kvlen: at least the longest
- * sequence's queries / keys (host values that size the grid).  head_dim at most 256.  16-bit tensors with
+ * sequence's queries / keys (host values that size the grid; the rows of a sequence behind its first max_seqlen are
+ * zero).  head_dim at most 256.  16-bit tensors with
  * head_dim a multiple of 8 up to 128, 16-byte aligned rows and at most 128 query heads per kv head run on the
  * tensor cores, other calls on a plain kernel.  fp32 softmax and sums; on the tensor cores the
  * probabilities are rounded to the inputs' type for the second product.
