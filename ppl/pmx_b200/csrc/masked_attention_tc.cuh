@@ -20,7 +20,7 @@
 // would idle split their keys too.
 //
 // On B200, bf16: 8192 causal tokens of 32/8 heads of 128 in 464 us, 1.18 PFLOP/s (72 % of the measured rate); without
-// the mask 950 us, 1.16 PFLOP/s; 32 trees of 16 tokens over 400 MB of cache in 92 us.
+// the mask 950 us, 1.16 PFLOP/s; 32 trees of 16 tokens over 400 MB of cache in 88 us.
 // The bound is the tensor pipe and, next to it, the exponentials: per 128 x 128 scores 1024 cycles of products (head
 // size 128) against 1024 of the special function unit, and a tile's softmax lies between its own two products.  So a
 // half's softmax runs beside the other half's products, and is kept short.  The running maximum moves only when a
@@ -56,6 +56,7 @@ struct TcArgs {
   float* part_o;
   float2* part_ml;
   int2* pieces;
+  int4* cuts;                               // of each CTA: the item it begins and others end: first token, rows, key head, last CTA
   int group, tokens;                        // query heads per key head, tokens of a row tile
   int row_blocks, splits, pair;
   int pieces_of_item;                       // about the most, from the host's lengths
@@ -346,6 +347,7 @@ struct Items {
       return;
     }
     const int lane = threadIdx.x & 31;
+    if (lane == 0 && (int)blockIdx.x < p.ctas) p.cuts[blockIdx.x] = make_int4(0, 0, 0, 0);
     int64_t sum = 0;
     Sequence q;
     for (int i = lane; i < a.B; i += 32) sum += tiles_of(p, i, q);
@@ -422,9 +424,11 @@ struct Items {
     w.tok0 = 0;
     finish_work(p, w, t0, t0 + take);
     w.slot = t0 > 0 ? 2 * (int)blockIdx.x : (take < tiles ? 2 * (int)blockIdx.x + 1 : -1);
-    if (t0 == 0 && (threadIdx.x & 31) == 0)       // the CTA that holds the first tile says who shares the item
-      p.pieces[(int64_t)b * a.Hkv + w.h] =
-          make_int2((int)blockIdx.x, (int)(((u + tiles) * ctas - 1) / total));
+    if (t0 == 0 && (threadIdx.x & 31) == 0) {     // the CTA that holds the first tile says who shares the item
+      const int last = (int)(((u + tiles) * ctas - 1) / total);
+      p.pieces[(int64_t)b * a.Hkv + w.h] = make_int2((int)blockIdx.x, last);
+      if (take < tiles) p.cuts[blockIdx.x] = make_int4((int)s.q0, s.n * p.group, w.h, last);
+    }
     u += take;
     return true;
   }
@@ -1215,8 +1219,10 @@ __global__ void __launch_bounds__(256) masked_attention_merge_kernel(const float
 }
 
 // The same for items whose key tiles were dealt out: WARPS warps per row share the pieces of its item.  One warp up to
-// four pieces, whose loads are all under way at once; beyond, a block, as a single warp would wait for memory once for every
-// four (one row over 100 000 keys, 148 pieces: 30 us, 48 us with one warp; eight drafted tokens over 12 000: 18 and 27).
+// four pieces, whose loads are all under way at once, for the rows of the at most one item that each CTA began and others
+// ended (looking up what each row of the call needs took 4 us more of 92 with 32 sequences, 40 of 178 with 128).
+// Beyond four pieces a block for every row, as a single warp would wait for memory once for every four (one row over 100 000
+// keys, 148 pieces: 30 us, 48 us with one warp; eight drafted tokens over 12 000: 18 and 27).
 template <typename T, int WARPS>
 __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid_constant__ TcArgs p) {
   __shared__ float4 shares[WARPS > 1 ? 8 : 1][32];
@@ -1226,24 +1232,36 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
   const AttnArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5, part = warp % WARPS;
-  const int64_t row = ((int64_t)blockIdx.x * 8 + warp) / WARPS, t = row / a.Hq;
-  if (t >= a.Tq) return;
-  // the row's sequence: the last that begins at or before it
-  int before = 0, start = 0;
-  for (int i = lane; i <= a.B; i += 32) {
-    const int64_t v = __ldcg(a.seqstarts + i);
-    if (v <= t) {
-      ++before;
-      start = v > start ? (int)v : start;
+  int2 who;
+  int r;
+  int64_t row;
+  if (WARPS == 1) {                                // rows of the item that a CTA began and others ended
+    const int4 cut = __ldcg(p.cuts + blockIdx.y);
+    r = (int)blockIdx.x * 8 + warp;
+    if (r >= cut.y) return;
+    who = make_int2((int)blockIdx.y, cut.w);
+    row = (int64_t)(cut.x + r / p.group) * a.Hq + cut.z * p.group + r % p.group;
+  } else {                                         // all rows
+    row = blockIdx.x;
+    const int64_t t = row / a.Hq;
+    // the row's sequence: the last that begins at or before it
+    int before = 0, start = 0;
+    for (int i = lane; i <= a.B; i += 32) {
+      const int64_t v = __ldcg(a.seqstarts + i);
+      if (v <= t) {
+        ++before;
+        start = v > start ? (int)v : start;
+      }
     }
+    const int b = __reduce_add_sync(0xFFFFFFFFu, before) - 1;
+    const int head = (int)(row - t * a.Hq), h = head / p.group;
+    const int64_t i = t - __reduce_max_sync(0xFFFFFFFFu, start);
+    if (b < 0 || b >= a.B || i >= a.max_seqlen) return;
+    who = __ldcg(p.pieces + (int64_t)b * a.Hkv + h);
+    if (who.x == who.y) return;                    // in one piece: the result is there
+    r = (int)i * p.group + head % p.group;
   }
-  const int b = __reduce_add_sync(0xFFFFFFFFu, before) - 1;
-  const int head = (int)(row - t * a.Hq), h = head / p.group;
-  const int64_t i = t - __reduce_max_sync(0xFFFFFFFFu, start);
-  if (b < 0 || b >= a.B || i >= a.max_seqlen) return;
-  const int2 who = __ldcg(p.pieces + (int64_t)b * a.Hkv + h);
-  if (who.x == who.y) return;                      // in one piece: the result is there
-  const int r = (int)i * p.group + head % p.group, n = who.y - who.x + 1;         // pieces, of which this warp takes every WARPS-th
+  const int n = who.y - who.x + 1;                 // pieces, of which this warp takes every WARPS-th
   auto place = [&](int c) { return (int64_t)(c == 0 ? 2 * who.x + 1 : 2 * (who.x + c)) * 128 + r; };
   auto stat = [&](int c) { return c < n ? __ldcg(p.part_ml + place(c)) : make_float2(-INFINITY, 0.f); };
   auto values = [&](int c) {
@@ -1344,13 +1362,15 @@ TcPlan plan_tc(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_
 
 // 16-byte aligned parts: maximum and sum, results, and who shares an item
 size_t tc_workspace(const TcPlan& pl, int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, size_t* o_at = nullptr,
-                    size_t* pieces_at = nullptr) {
+                    size_t* pieces_at = nullptr, size_t* cuts_at = nullptr) {
   if (!pl.use || (pl.splits == 1 && !pl.flat)) return 0;
   const size_t rows = pl.flat ? (size_t)pl.grid * 2 * kTile : (size_t)pl.splits * Tq * Hq;
   const size_t o = (rows * sizeof(float2) + 15) & ~(size_t)15, pieces = o + rows * D * sizeof(float);
   if (o_at) *o_at = o;
   if (pieces_at) *pieces_at = pieces;
-  return pieces + (pl.flat ? (size_t)B * Hkv * sizeof(int2) : 0);
+  const size_t cuts = (pieces + (size_t)B * Hkv * sizeof(int2) + 15) & ~(size_t)15;
+  if (cuts_at) *cuts_at = cuts;
+  return pl.flat ? cuts + (size_t)pl.grid * sizeof(int4) : pieces;
 }
 
 bool rows_ok_for_tma(const void* base, int64_t row, int64_t head, int64_t rows) {
@@ -1387,7 +1407,8 @@ int launch_tc_t(const TileMaps& maps, const TcArgs& p, int grid, cudaStream_t s)
   const dim3 merge_grid((unsigned)ceil_div(rows, 8)), merge_block(256);
   if (p.flat && p.pieces_of_item > 4 && p.a.Tq * p.a.Hq < (1ll << 31))      // a block per row
     return launch_pdl_k(masked_attention_join_kernel<T, 8>, dim3((unsigned)(p.a.Tq * p.a.Hq)), merge_block, 0, s, p);
-  if (p.flat) return launch_pdl_k(masked_attention_join_kernel<T, 1>, merge_grid, merge_block, 0, s, p);
+  const int64_t most = (int64_t)p.a.max_seqlen * p.group;          // rows of an item
+  if (p.flat) return launch_pdl_k(masked_attention_join_kernel<T, 1>, dim3((unsigned)ceil_div(most < kTile ? most : kTile, 8), (unsigned)p.ctas), merge_block, 0, s, p);
   return launch_pdl_k(masked_attention_merge_kernel<T>, merge_grid, merge_block, 0, s, (const float*)p.part_o,
                       (const float2*)p.part_ml, (T*)p.a.out, rows, p.a.D, p.splits);
 }
@@ -1411,11 +1432,12 @@ int launch_tc(const AttnArgs& a, const TcPlan& pl, int dtype, const char* name, 
   p.pieces_of_item = pl.pieces;
   int64_t grid = pl.grid;
   if (a.tree_mask && grid < ceil_div(a.Tq, 2)) grid = ceil_div(a.Tq, 2) < sm_count() ? ceil_div(a.Tq, 2) : sm_count();
-  size_t o_at = 0, pieces_at = 0;
-  tc_workspace(pl, a.Tq, a.B, a.Hq, a.Hkv, a.D, &o_at, &pieces_at);
+  size_t o_at = 0, pieces_at = 0, cuts_at = 0;
+  tc_workspace(pl, a.Tq, a.B, a.Hq, a.Hkv, a.D, &o_at, &pieces_at, &cuts_at);
   p.part_ml = reinterpret_cast<float2*>(ws);
   p.part_o = reinterpret_cast<float*>((char*)ws + o_at);
   p.pieces = reinterpret_cast<int2*>((char*)ws + pieces_at);
+  p.cuts = reinterpret_cast<int4*>((char*)ws + cuts_at);
   TileMaps m{};
   int st = make_head_map(&m.q, a.q, a.Tq, a.Hq, a.D, a.q_tok, a.q_head, (uint32_t)pl.group, (uint32_t)pl.tokens, dtype, name);
   if (st == PMX_OK) st = make_head_map(&m.k, a.past.k, a.past.rows, a.Hkv, a.D, a.past.k_row, a.past.k_head, 1, kTile, dtype, name);
