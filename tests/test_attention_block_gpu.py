@@ -600,3 +600,54 @@ def test_calls_that_need_converting_give_the_same_as_regular_ones(DB):
         assert eq(DB.rotary_position_embedding(q.clone().requires_grad_(), k, ss, sp), DB.rotary_position_embedding(q, k, ss, sp))
     with pytest.raises(Exception, match="backward|derivative|grad"):
         DB.rotary_position_embedding(q.clone().requires_grad_(), k, ss, sp)[0].sum().backward()
+
+
+def test_graphs_and_streams_side_by_side(DB):
+    """Two captured calls with workspaces of their own, replayed in turn with other inputs, and eager calls on two streams."""
+    rng = np.random.default_rng(31)
+    Hq, Hkv, D = 8, 2, 128
+    q = [dev(values(rng, (4, Hq, D), "bf16"), "bf16") for _ in range(4)]
+    k = dev(values(rng, (3000, Hkv, D), "bf16"), "bf16")
+    call = lambda x, keys: DB.prompt_attention(x, k[:keys], k[:keys], i64([0, 4]), i64([0, keys]), 4, keys, Hq, D,  # noqa: E731
+                                               num_kv_heads=Hkv)
+    want = [[call(x, keys) for keys in (3000, 1700)] for x in q]
+    ss, ends, static = i64([0, 4]), {n: i64([0, n]) for n in (3000, 1700)}, q[0].clone()
+    graphs, outs = [], []
+    for keys in (3000, 1700):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=graphs[0].pool() if graphs else None):
+            outs.append(DB.prompt_attention(static, k[:keys], k[:keys], ss, ends[keys], 4, keys, Hq, D, num_kv_heads=Hkv))
+        graphs.append(graph)
+    for i, x in enumerate(q):
+        static.copy_(x)
+        for g in ((0, 1), (1, 0))[i % 2]:
+            graphs[g].replay()
+            assert torch.equal(outs[g], want[i][g])
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for side in sides:
+        side.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for n, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[n].append(call(q[n], 3000))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[n][0]) for n in range(2) for x in got[n])
+
+
+def test_tree_attention_drops_what_is_behind_max_seqlen_and_outside_the_cache(DB):
+    """Rows of a sequence behind its first max_seqlen are zero and not stored; rows beyond the cache's end are not stored."""
+    rng = np.random.default_rng(32)
+    Hq, Hkv, D, rows = 4, 2, 64, 40
+    cache_np = values(rng, (rows, 1, 2, Hkv, D), "f16")
+    q, k, v = (values(rng, (12, h, D), "f16") for h in (Hq, Hkv, Hkv))
+    masks = np.array([(1 << (i % 6 + 1)) - 1 for i in range(12)], dtype=np.int64)
+    cache = dev(cache_np, "f16")
+    got = DB.tree_cache_attention(dev(q, "f16"), dev(k, "f16"), dev(v, "f16"), i64([0, 6, 12]), i64([0, 20]), i64([5, 18]),
+                                  i64(masks), 4, 30, cache, Hq, D, num_kv_heads=Hkv)
+    keep = np.array([0, 1, 2, 3, 6, 7, 8, 9])
+    want = cache_np.copy()
+    ref = ab.tree_attention(q[keep], k[keep], v[keep], want, 0, 0, [0, 4, 8], [0, 20], [5, 18], masks[keep], 1 / 8.0)
+    check_attention(got[torch.from_numpy(keep).cuda()], ref, "f16", D, 30, 0.0)
+    assert not got[torch.tensor([4, 5, 10, 11], device="cuda")].any()
+    assert np.array_equal(host(cache), want)
