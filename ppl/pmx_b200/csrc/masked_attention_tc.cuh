@@ -1093,7 +1093,9 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
       const int total = tiles_of(w);
       const bool row_ok = row.ok;
       const int64_t out_row = (w.s.q0 + row.tok) * a.Hq + row.head;
-      const bool bad = ctl->bad[place] == w.number;
+      // Whether a value was replaced is known once the products of ALL of a row's tiles are done: here where a row's tiles
+      // belong to one half, behind the meeting of the halves where they share them.
+      bool bad = ctl->bad[place] == w.number;
       auto store = [&](Cols8& x, int col, float inv, float* part) {       // 8 columns of this row
         if (bad) x = add_bad<T>(x, &a, &w, col, row.limit, row.bits, total);
         if (!part) {
@@ -1140,6 +1142,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         ok = !named_any(4, 256, !ok);
         if (!ok) break;
         tc_fence_after();
+        bad = ctl->bad[place] == w.number;
         const float2 other = ctl->ml[(half ^ 1) * 128 + r];
         const float top = fmaxf(m, other.x);
         const float f0 = m == -INFINITY ? 0.f : ex2(m - top), f1 = other.x == -INFINITY ? 0.f : ex2(other.x - top);
