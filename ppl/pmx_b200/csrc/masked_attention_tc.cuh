@@ -916,7 +916,13 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         float* x = reinterpret_cast<float*>(raw);
         tmem_ld32(s_tmem + c * 32, raw);
         tmem_wait_ld32(raw);
+        const uint32_t bits = c < 2 ? (c == 0 ? seen[0] : seen[1]) : (c == 2 ? seen[2] : seen[3]);
         if (a.cap > 0.f) {
+          // scores that the row may not see, NaN among them, stay out of what follows: neighbours share a reciprocal
+          if (bits != 0xFFFFFFFFu) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = bits & (1u << j) ? x[j] : 0.f;
+          }
           float big = 0.f;
 #pragma unroll
           for (int j = 0; j < 32; j += 2) big = max3(big, fabsf(x[j]), fabsf(x[j + 1]));
@@ -966,7 +972,6 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
             for (int j = 0; j < 32; ++j) x[j] = fmaf(-slope2, fabsf(at - (float)j), x[j] * one);
           }
         }
-        const uint32_t bits = c < 2 ? (c == 0 ? seen[0] : seen[1]) : (c == 2 ? seen[2] : seen[3]);
         if (bits != 0xFFFFFFFFu) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) x[j] = bits & (1u << j) ? x[j] : -INFINITY;

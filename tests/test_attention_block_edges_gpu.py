@@ -1,10 +1,13 @@
 """The attention block's operators on the GPU where they are easiest to get wrong."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
+from oracle import attention_block as ab
 from tests.helpers import dev
-from tests.test_attention_block_gpu import DB, cache_of, i64, no_wait_ran_out, prompt_case, values  # noqa: F401
+from tests.test_attention_block_gpu import DB, cache_of, check_attention, i64, no_wait_ran_out, prompt_case, values  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +74,67 @@ def test_bad_values_of_drafted_trees_reach_all_columns(DB, kind, dtype, D, past)
             bad[3 + j, 0, 1, :, col] = x
             for _ in range(4):
                 only_its_column(run(v, bad.clone()), clean, list(range(n)), col, is_kind)
+
+
+# ------------------------------------------------------------------------------- hidden content under a cap, a bias, a prefix
+SCORES = {"cap": dict(cap=0.7), "high_cap": dict(cap=40.0), "bias": dict(alibi=True), "prefix": dict(prefix=[33, 8]),
+          "all": dict(cap=5.0, alibi=True, prefix=[33, 9])}
+HIDDEN = [float("nan"), float("inf"), float("-inf"), 300.0]
+
+
+def hidden_prompt(DB, dtype, Hq, Hkv, D, lens, scores, seed=5):
+    """-> clean call, its reference, and run(key, value, query)"""
+    rng = np.random.default_rng(seed)
+    cap, prefix = scores.get("cap", 0.0), scores.get("prefix")
+    q, k, v, ss, ks, ms, mk = prompt_case(rng, lens, Hq, Hkv, D, dtype, 9)
+    slopes = (2.0 ** (-8.0 * (np.arange(Hq) + 1) / Hq)).astype(np.float32) if scores.get("alibi") else None
+    tq, tk, tv = dev(q, dtype), dev(k, dtype), dev(v, dtype)
+
+    def run(tq=tq, tk=tk, tv=tv):
+        return DB.prompt_attention(tq, tk, tv, i64(ss), i64(ks), ms, mk, Hq, D, num_kv_heads=Hkv, logit_cap=cap,
+                                   alibi_slopes=None if slopes is None else torch.from_numpy(slopes).cuda(),
+                                   prefix_lens=None if prefix is None else i64(prefix))
+    ref = ab.prompt_attention(q, k, v, ss, ks, True, 1 / math.sqrt(D), cap, slopes, prefix)
+    return run, ref, (tq, tk, tv), mk, cap
+
+
+@pytest.mark.parametrize("bad", HIDDEN)
+@pytest.mark.parametrize("scores", sorted(SCORES))
+@pytest.mark.parametrize("dtype,Hq,Hkv,D", [("bf16", 4, 2, 128), ("f16", 3, 1, 64), ("f16", 6, 1, 64), ("f32", 2, 1, 32)])
+@pytest.mark.parametrize("n,L", [(70, 200), (70, 201), (9, 131), (9, 132)])
+def test_hidden_content_with_scores_of_every_kind(DB, bad, scores, dtype, Hq, Hkv, D, n, L):
+    """Hidden keys and values at odd and even places, next to visible ones: later tokens, the next sequence, behind the last."""
+    lens = [(n, L), (8, 64)]
+    run, ref, (tq, tk, tv), mk, cap = hidden_prompt(DB, dtype, Hq, Hkv, D, lens, SCORES[scores])
+    for j in (L - n + 4, L - n + 5, L - 1, L, L + 64):
+        kk, vv = tk.clone(), tv.clone()
+        kk[j], vv[j] = bad, bad
+        if j < L:
+            sees = [i for i in range(n) if i + L - n >= j]
+        else:
+            sees = list(range(n, n + 8)) if j == L else []
+        blind = [t for t in range(n + 8) if t not in sees]
+        got = run(tk=kk, tv=vv)
+        check_attention(got[blind], tuple(x[blind] for x in ref), dtype, D, mk, cap, dtype != "f32")
+        if sees and not math.isfinite(bad):
+            assert not torch.isfinite(got[sees]).any()
+
+
+@pytest.mark.parametrize("bad", HIDDEN)
+@pytest.mark.parametrize("cap", [0.0, 0.7, 40.0])
+@pytest.mark.parametrize("past", [130, 131, 0])
+def test_hidden_rows_and_siblings_with_a_cap(DB, bad, cap, past):
+    rng = np.random.default_rng(past)
+    Hq, Hkv, D, n, dtype = 6, 2, 64, 7, "f16"
+    cache_np = cache_of(rng, 0, 200, 1, Hkv, D, dtype)
+    q, k, v = (values(rng, (n, h, D), dtype) for h in (Hq, Hkv, Hkv))
+    mask = np.array([0b1, 0b11, 0b101, 0b1001, 0b10101, 0b100011, 0b1000001], np.int64)
+    ref = ab.tree_attention(q, k, v, cache_np.copy(), 0, 0, [0, n], [20], [past], mask, 1 / math.sqrt(D), cap)
+    for token, sees in ((1, [1, 5]), (2, [2, 4]), (3, [3])):
+        cache, kk, vv = dev(cache_np, dtype), dev(k, dtype), dev(v, dtype)
+        cache[:20], cache[20 + past:] = bad, bad
+        kk[token], vv[token] = bad, bad
+        got = DB.tree_cache_attention(dev(q, dtype), kk, vv, i64([0, n]), i64([20]), i64([past]), i64(mask), n, past + n, cache, Hq, D,
+                                      num_kv_heads=Hkv, logit_cap=cap)
+        blind = [t for t in range(n) if t not in sees]
+        check_attention(got[blind], tuple(x[blind] for x in ref), dtype, D, past + n, cap)
