@@ -227,6 +227,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {     // NaN wi
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ float max3_number(float a, float b, float c) {     // NaN loses
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -896,7 +901,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
     // in a loop that is not unrolled, run only where there is something to do: the hot loop is as long as the instruction
     // caches can bear (8192 capped tokens, otherwise alike: 961 us so, 1184 us with the same arithmetic unrolled in it; code that
     // was merely skipped cost a fifth).
-    auto adjust = [&](const Work& w, int t, int whole, float slope2, float place_of_row) {
+    auto adjust = [&](const Work& w, int t, int whole, float slope2, float place_of_row, float to_vote) {
       uint32_t seen[4] = {0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu};
       if (t >= whole) {
         const Row row = row_of(w);
@@ -918,22 +923,36 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         tmem_wait_ld32(raw);
         const uint32_t bits = c < 2 ? (c == 0 ? seen[0] : seen[1]) : (c == 2 ? seen[2] : seen[3]);
         if (a.cap > 0.f) {
-          // scores that the row may not see, NaN among them, stay out of what follows: neighbours share a reciprocal
-          if (bits != 0xFFFFFFFFu) {
+          auto largest = [&]() {             // NaN left out
+            float big = 0.f;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = bits & (1u << j) ? x[j] : 0.f;
+            for (int j = 0; j < 32; j += 2) big = max3_number(big, fabsf(x[j]), fabsf(x[j + 1]));
+            return big;
+          };
+          // The warp votes for a form by what its rows see.  The forms round differently, so what a row may not see must not
+          // count, nor lanes without a row, which hold the next sequence's or what was in shared memory before (their to_vote
+          // is 0).  And the last form's scores share a reciprocal, through which a hidden NaN would reach a visible one.
+          // Both are seen to where the vote is not for the short form at once, out of the usual way (32 capped trees of 16
+          // over 4096 rows: 110 us without it, 116 so, 119 with all hidden scores set to zero first; 8192 capped tokens: 726,
+          // 734, 740).  Each row by itself would leave its neighbours out too, but takes a third longer near the cap.
+          float big = largest();
+          bool near = __all_sync(0xFFFFFFFFu, !(big * to_vote > 0.4f));
+          if (!near) {
+            if (bits != 0xFFFFFFFFu) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] = bits & (1u << j) ? x[j] : 0.f;
+              big = largest();
+            }
+            near = __all_sync(0xFFFFFFFFu, !(big * to_vote > 0.4f));
           }
-          float big = 0.f;
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) big = max3(big, fabsf(x[j]), fabsf(x[j + 1]));
-          if (__all_sync(0xFFFFFFFFu, big * to_y <= 0.4f)) {
+          if (near) {
             // |s| <= 0.4 c, as almost everywhere: the short polynomial (8192 capped tokens: 755 us, 835 us without it)
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               const f32x2 xx = pair2(x[j], x[j + 1]);
               unpair2(mul2(mul2(xx, pair2(sl2, sl2)), tanh_over_y_near(mul2(xx, pair2(to_y, to_y)))), x[j], x[j + 1]);
             }
-          } else if (__all_sync(0xFFFFFFFFu, big * to_y <= 1.0f)) {
+          } else if (__all_sync(0xFFFFFFFFu, !(big * to_vote > 1.0f))) {
             // tanh by its polynomial, off the special function unit
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
@@ -996,6 +1015,8 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         if (row.ok) slope2 = __ldcg(a.slopes + row.head) * kLog2e;
         place_of_row = (float)(row.tok + w.s.shift - (int64_t)w.t0 * kTile);
       }
+      // s / c of a product, for the vote in adjust(): 0 in lanes without a row
+      const float to_vote = r < rows_tile && w.tok0 + (p.pair ? half * p.tokens : 0) + row_tok < w.s.n ? to_y : 0.f;
       float m = -INFINITY, l = 0.f;                                   // m: in log2 domain
       const int t_step = p.pair ? 1 : 2;
       int t = w.t0 + (p.pair ? 0 : half);
@@ -1006,7 +1027,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         tc_fence_after();
         const float at = place_of_row - (float)((t - w.t0) * kTile);      // the row, from the tile's first key
         const bool linear = BIAS && a.cap == 0.f && t < whole && __all_sync(0xFFFFFFFFu, at >= (float)(kTile - 1));
-        if ((score && !linear) || t >= whole) adjust(w, t, whole, slope2, place_of_row);
+        if ((score && !linear) || t >= whole) adjust(w, t, whole, slope2, place_of_row, to_vote);
         uint32_t raw[128];
         float* x = reinterpret_cast<float*>(raw);
 #pragma unroll

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import attention_block as ab
-from tests.helpers import dev
+from tests.helpers import TORCH_DT, dev
 from tests.test_attention_block_gpu import DB, cache_of, check_attention, i64, no_wait_ran_out, prompt_case, values  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +138,30 @@ def test_hidden_rows_and_siblings_with_a_cap(DB, bad, cap, past):
                                       num_kv_heads=Hkv, logit_cap=cap)
         blind = [t for t in range(n) if t not in sees]
         check_attention(got[blind], tuple(x[blind] for x in ref), dtype, D, past + n, cap)
+
+
+# ------------------------------------------------------------------------------- bits of a capped row
+@pytest.mark.parametrize("dtype,Hq,Hkv,D", [("f16", 4, 2, 64), ("f16", 3, 1, 64), ("f16", 12, 1, 128)])
+@pytest.mark.parametrize("cap", [2.0, 300.0])
+@pytest.mark.parametrize("n,L", [(70, 201), (9, 131)])
+def test_bits_of_a_capped_row_do_not_depend_on_hidden_content(DB, dtype, Hq, Hkv, D, cap, n, L):
+    """Neither hidden keys nor the rows of another sequence, nor what other calls left behind, change a result by a bit.  (Rows
+    of the same sequence may: those that share a warp take the same form of tanh.)"""
+    run, _, (tq, tk, tv), _, _ = hidden_prompt(DB, dtype, Hq, Hkv, D, [(n, L), (8, 64)], dict(cap=cap))
+    clean = run()
+    for x in (float("nan"), 400.0):
+        for j in (L - 1, L, L + 64):
+            kk = tk.clone()
+            kk[j] = x
+            blind = list(range(n, n + 8) if j < L else range(n if j == L else n + 8))
+            assert torch.equal(run(tk=kk)[blind], clean[blind])
+        for t in (0, n - 1, n, n + 8):
+            qq = tq.clone()
+            qq[t] = x
+            blind = list(range(n, n + 8) if t < n else range(n if t == n else n + 8))
+            assert torch.equal(run(tq=qq)[blind], clean[blind])
+    for x in (float("nan"), 400.0, 0.0):                        # what another call leaves in the SM's memory
+        filler = torch.full((4096, 4, D), x, device="cuda", dtype=TORCH_DT[dtype])
+        DB.prompt_attention(filler, filler, filler, i64([0, 4096]), i64([0, 4096]), 4096, 4096, 4, D)
+        got = run()
+        assert torch.equal(got[:n + 8], clean[:n + 8])
