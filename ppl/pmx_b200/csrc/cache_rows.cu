@@ -20,6 +20,7 @@ struct CompactArgs {
   int64_t rows, index_count;
   int64_t row_bytes, layer_bytes, kv_bytes, head_bytes;   // strides
   int layers, heads, chunks;                              // chunks: vectors of a head row
+  int max_accept;                                         // of a sequence; the kernel's variant has vectors for as many rows
 };
 
 constexpr int kWarps = 8;
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(kWarps * 32) compact_cache_kernel(const __grid
   if (warp == 0) {
     const int64_t first = __ldcg(a.accept_starts + b), last = __ldcg(a.accept_starts + b + 1);
     const int64_t base = __ldcg(a.cachestarts + b) + __ldcg(a.start_pos + b);
-    const int64_t n = first < 0 || last > a.index_count ? 0 : (last - first < R * kVectors ? last - first : R * kVectors);
+    const int64_t n = first < 0 || last > a.index_count ? 0 : (last - first < a.max_accept ? last - first : a.max_accept);
     int before = 0;
     for (int i = lane; i < kMaxAccept; i += 32) {
       const int64_t from = i < n ? __ldcg(a.accept_index + first + i) : -1;
@@ -94,15 +95,15 @@ __global__ void __launch_bounds__(kWarps * 32) compact_cache_kernel(const __grid
 }
 
 template <typename VEC>
-int launch_compact_vec(const CompactArgs& a, int max_accept, int64_t B, cudaStream_t s) {
+int launch_compact_vec(const CompactArgs& a, int64_t B, cudaStream_t s) {
   // 16 columns side by side are the 256 bytes of a usual head's row; more rows than 16 take twice the registers, more
   // than 32 half the columns.  Up to eight blocks per SM: 26 and 27 us in the case above with twelve and sixteen.
-  const int w = max_accept <= 32 ? 16 : 8;
+  const int w = a.max_accept <= 32 ? 16 : 8;
   const int64_t blocks = ceil_div(ceil_div((int64_t)a.layers * 2 * a.heads * a.chunks, w), kWarps);
   const int64_t most = ceil_div((int64_t)sm_count() * 8, B);
   const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)B), block(kWarps * 32);
-  if (max_accept <= 16) return launch_pdl_k(compact_cache_kernel<VEC, 16, 8>, grid, block, 0, s, a);
-  if (max_accept <= 32) return launch_pdl_k(compact_cache_kernel<VEC, 16, 16>, grid, block, 0, s, a);
+  if (a.max_accept <= 16) return launch_pdl_k(compact_cache_kernel<VEC, 16, 8>, grid, block, 0, s, a);
+  if (a.max_accept <= 32) return launch_pdl_k(compact_cache_kernel<VEC, 16, 16>, grid, block, 0, s, a);
   return launch_pdl_k(compact_cache_kernel<VEC, 8, 16>, grid, block, 0, s, a);
 }
 
@@ -117,7 +118,6 @@ int launch_compact_cache(const pmx_compact_cache_args& p, cudaStream_t s) {
   if (p.max_accept > 64) return fail(PMX_ERR_UNSUPPORTED, "compact_cache: at most 64 accepted rows a sequence");
   if (p.sequences > 65535 || p.num_layers > (1 << 20) || p.num_kv_heads > (1 << 20) || p.head_dim > (1 << 20))
     return fail(PMX_ERR_UNSUPPORTED, "compact_cache: sizes beyond what the kernel indexes");
-  const int max_accept = (int)p.max_accept;
   int e;
   switch (p.dtype) {
     case PMX_DTYPE_F16: case PMX_DTYPE_BF16: e = 2; break;
@@ -131,15 +131,15 @@ int launch_compact_cache(const pmx_compact_cache_args& p, cudaStream_t s) {
   CompactArgs a{};
   a.cache = (char*)p.cache;
   a.cachestarts = p.cachestarts; a.start_pos = p.start_pos; a.accept_starts = p.accept_starts; a.accept_index = p.accept_index;
-  a.rows = p.cache_rows; a.index_count = p.index_count;
+  a.rows = p.cache_rows; a.index_count = p.index_count; a.max_accept = (int)p.max_accept;
   a.row_bytes = p.row_stride * e; a.layer_bytes = p.layer_stride * e; a.kv_bytes = p.kv_stride * e; a.head_bytes = p.head_stride * e;
   a.layers = (int)p.num_layers; a.heads = (int)p.num_kv_heads; a.chunks = (int)p.head_dim * e / vec;
   if (p.num_layers * 2 * p.num_kv_heads >= (1 << 30) / a.chunks) return fail(PMX_ERR_UNSUPPORTED, "compact_cache: cache too wide");
   switch (vec) {
-    case 16: return launch_compact_vec<uint4>(a, max_accept, p.sequences, s);
-    case 8: return launch_compact_vec<uint2>(a, max_accept, p.sequences, s);
-    case 4: return launch_compact_vec<uint32_t>(a, max_accept, p.sequences, s);
-    default: return launch_compact_vec<uint16_t>(a, max_accept, p.sequences, s);
+    case 16: return launch_compact_vec<uint4>(a, p.sequences, s);
+    case 8: return launch_compact_vec<uint2>(a, p.sequences, s);
+    case 4: return launch_compact_vec<uint32_t>(a, p.sequences, s);
+    default: return launch_compact_vec<uint16_t>(a, p.sequences, s);
   }
 }
 

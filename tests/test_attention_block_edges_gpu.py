@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import attention_block as ab
-from tests.helpers import TORCH_DT, dev
+from tests.helpers import TORCH_DT, dev, host
 from tests.test_attention_block_gpu import DB, cache_of, check_attention, i64, no_wait_ran_out, prompt_case, values  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -165,3 +165,16 @@ def test_bits_of_a_capped_row_do_not_depend_on_hidden_content(DB, dtype, Hq, Hkv
         DB.prompt_attention(filler, filler, filler, i64([0, 4096]), i64([0, 4096]), 4096, 4096, 4, D)
         got = run()
         assert torch.equal(got[:n + 8], clean[:n + 8])
+
+
+# ------------------------------------------------------------------------------- compaction
+@pytest.mark.parametrize("most,listed", [(3, 12), (10, 12), (16, 20), (20, 40), (64, 70), (32, 33)])
+def test_compaction_moves_no_more_than_max_accept(DB, most, listed):
+    rng = np.random.default_rng(most)
+    cache = cache_of(rng, 1, 200, 2, 2, 16, "f16")
+    picks = rng.permutation(listed)
+    t = dev(cache, "f16")
+    DB.compact_cache(t, i64([5, 100]), i64([3, 2]), i64([0, listed, listed + 2]), i64(list(picks) + [1, 0]), most, num_layer=2,
+                     cache_layout=1)
+    ab.compact_cache(cache, 1, [5, 100], [3, 2], [0, most, most + 2], list(picks[:most]) + [1, 0])
+    assert np.array_equal(host(t), cache)
