@@ -3,7 +3,7 @@
 // A decode step launches kernels that run for 2 to 10 us; checking arguments, allocating results and packing
 // the argument struct in Python takes about as long again.  These functions do that for calls in which nothing needs
 // converting -- tensors on the current CUDA device, index arrays dense and 64 bits wide, views that the kernels
-// read in place, no gradient asked for, no export under way -- and call the C ABI (include/pmx_moe.h).  For any other
+// read in place, no gradient and no tangent asked for, no export under way -- and call the C ABI (include/pmx_moe.h).  For any other
 // call they return None, and the operators in torch_function/dynamic_batching check, convert and raise as they would
 // without this file.  A failed call comes back as its status.
 #define PY_SSIZE_T_CLEAN
@@ -46,7 +46,7 @@ struct Call {
       return nullptr;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
-    if (!t.is_cuda() || (grad && t.requires_grad())) {
+    if (!t.is_cuda() || (grad && t.requires_grad()) || t._fw_grad(0).defined()) {
       regular = false;
       return nullptr;
     }

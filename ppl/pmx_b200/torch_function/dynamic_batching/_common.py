@@ -5,6 +5,7 @@ import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from ..._cabi import lib
 
@@ -81,13 +82,18 @@ def host_int(name: str, key: str, v) -> int:
     return n
 
 
+def has_tangent(t) -> bool:
+    """Whether a tensor carries a tangent of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def wants_grad(*tensors) -> bool:
-    """The operators have no backward pass: where a gradient would be asked for they go through
-    autograd, which then says so, instead of returning results that silently carry none."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
+    """The operators have no backward pass and no tangents: where a gradient or a tangent would be asked for they go
+    through autograd, which then says so, instead of returning results that silently carry none."""
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and ((grad and t.requires_grad) or has_tangent(t)):
+            return True
     return False
 
 

@@ -4,7 +4,7 @@ from __future__ import annotations
 import torch
 
 from ..._cabi import lib, check, COMPACT_CACHE_ARGS, DTYPE_CODE
-from ._common import cache_strides, host, host_int, index, on_device, raw_stream, same_device
+from ._common import cache_strides, host, host_int, index, on_device, raw_stream, same_device, wants_grad
 
 
 def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: torch.Tensor, accept_starts: torch.Tensor,
@@ -29,8 +29,8 @@ def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: tor
     code = DTYPE_CODE.get(cache.dtype)
     if code is None:
         raise TypeError(f"{name}: dtype {cache.dtype} is not supported (float16, bfloat16, float32)")
-    if cache.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name}: changes the cache in place and has no backward pass")
+    if wants_grad(cache):
+        raise RuntimeError(f"{name}: changes the cache in place and has no backward pass and no forward-mode derivative")
     _, row_stride, kv_stride, head_stride, rows = cache_strides(cache, cache_layout, num_layer, 0)
     layer_stride = cache.stride(1 if cache_layout == 0 else 0)
     kv_heads = cache.shape[2 if cache_layout == 3 else 3]

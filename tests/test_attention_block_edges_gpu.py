@@ -178,3 +178,35 @@ def test_compaction_moves_no_more_than_max_accept(DB, most, listed):
                      cache_layout=1)
     ab.compact_cache(cache, 1, [5, 100], [3, 2], [0, most, most + 2], list(picks[:most]) + [1, 0])
     assert np.array_equal(host(t), cache)
+
+
+# ------------------------------------------------------------------------------- tangents, memory, workspaces
+def every_operator(DB, q, k, v, w, cache, indices):
+    ss, z = i64([0, 5]).to(indices), i64([0])
+    D, H = q.shape[2], q.shape[1]
+    return {"rotary": lambda: DB.rotary_position_embedding(q, k, ss, z),
+            "norm": lambda: DB.qk_norm_rotary_embedding(q, k, w, w, 1e-6, ss, z),
+            "prompt": lambda: DB.prompt_attention(q, k, v, ss, ss, 5, 5, H, D),
+            "tree": lambda: DB.tree_cache_attention(q, k, v, ss, z, z, i64([1] * 5), 5, 5, cache, H, D),
+            "compact": lambda: DB.compact_cache(cache, z, z, i64([0, 2]).to(indices), i64([1, 2]), 2)}
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("indices", [torch.int64, torch.int32])
+def test_a_tangent_is_refused_not_dropped(DB, which, indices):
+    import torch.autograd.forward_ad as fw
+    t = [torch.randn(5, 2, 64, device="cuda") for _ in range(3)] + [torch.randn(64, device="cuda"),
+                                                                     torch.randn(9, 1, 2, 2, 64, device="cuda")]
+    uses = {"rotary": (0, 1), "norm": (0, 1, 3), "prompt": (0, 1, 2), "tree": (0, 1, 2, 4), "compact": (4,)}
+    with fw.dual_level():
+        x = list(t)
+        x[which] = fw.make_dual(t[which], torch.ones_like(t[which]))
+        for name, call in every_operator(DB, *x, indices).items():
+            if which in uses[name]:
+                with pytest.raises((RuntimeError, NotImplementedError), match="jvp|forward|backward"):
+                    call()
+            else:
+                call()
+    q = t[0]
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda x: every_operator(DB, x, *t[1:], indices)["prompt"](), (q,), (q,))
