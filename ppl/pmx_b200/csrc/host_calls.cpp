@@ -12,6 +12,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -116,15 +117,13 @@ at::Tensor dense_like(const at::Tensor& t) {
 }
 PyObject* none() { Py_RETURN_NONE; }
 
-// no C++ exception leaves for the interpreter
+// no C++ exception leaves for the interpreter: each becomes the one that torch raises for it (running out of memory is
+// torch.OutOfMemoryError)
 template <PyObject* (*F)(PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  try {
-    return F(args, n);
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+  HANDLE_TH_ERRORS
+  return F(args, n);
+  END_HANDLE_TH_ERRORS
 }
 
 // cache [5 dimensions] in one of the four layouts -> strides and sizes, or false

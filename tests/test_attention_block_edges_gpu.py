@@ -210,3 +210,10 @@ def test_a_tangent_is_refused_not_dropped(DB, which, indices):
     q = t[0]
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.func.jvp(lambda x: every_operator(DB, x, *t[1:], indices)["prompt"](), (q,), (q,))
+
+
+def test_running_out_of_memory_says_so(DB):
+    q = torch.zeros(1, 1, 128, device="cuda", dtype=torch.float16).expand(1 << 30, 1, 128)      # a result of 256 GB
+    for ss in (i64([0, 1 << 30]), i64([0, 1 << 30]).int()):
+        with pytest.raises(torch.OutOfMemoryError):
+            DB.rotary_position_embedding(q, None, ss, i64([0]))
