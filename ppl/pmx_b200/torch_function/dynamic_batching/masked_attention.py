@@ -8,7 +8,6 @@ merge where a long key axis is split because there are few rows.
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import math
 from typing import Optional
 
@@ -35,10 +34,6 @@ def _numbers(name: str, num_heads: int, kv_heads: int, head_dim: int, scale, log
     if not (logit_cap >= 0.0 and math.isfinite(logit_cap)):
         raise ValueError(f"{name}: logit_cap must be finite and not negative (0: no cap), not {logit_cap}")
     return scale
-
-
-# bytes of workspace by sizes; the GPU (they depend on its number of SMs) is the process's kind of GPU
-_workspace_bytes = functools.lru_cache(maxsize=1024)(lib.pmx_attention_workspace_bytes)
 
 
 def attention_check(device=None) -> None:
@@ -86,7 +81,7 @@ def _prompt(query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_h
     k0, k1, _ = k.stride()
     v0, v1, _ = v.stride()
     with on_device(dev):
-        nbytes = _workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen, max_kvlen, code)
+        nbytes = lib.pmx_attention_workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen, max_kvlen, code)
         ws = workspace(nbytes, q.device) if nbytes else None
         check(lib.pmx_prompt_attention(PROMPT_ATTENTION_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), seqstarts.data_ptr(), kvstarts.data_ptr(),
@@ -132,7 +127,7 @@ def _tree(query, current_key, current_value, seqstarts, cachestarts, start_pos, 
     k0, k1, _ = k.stride()
     v0, v1, _ = v.stride()
     with on_device(dev):
-        nbytes = _workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen, max_kvlen, code)
+        nbytes = lib.pmx_attention_workspace_bytes(Tq, B, num_heads, kv_heads, head_dim, max_seqlen, max_kvlen, code)
         ws = workspace(nbytes, q.device) if nbytes else None
         check(lib.pmx_tree_cache_attention(TREE_ATTENTION_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), cache.data_ptr(), seqstarts.data_ptr(), cachestarts.data_ptr(),

@@ -217,3 +217,21 @@ def test_running_out_of_memory_says_so(DB):
     for ss in (i64([0, 1 << 30]), i64([0, 1 << 30]).int()):
         with pytest.raises(torch.OutOfMemoryError):
             DB.rotary_position_embedding(q, None, ss, i64([0]))
+
+
+def test_workspace_is_asked_for_at_every_call(DB, monkeypatch):
+    """Its size goes by the current device: no answer is kept for a call on another one."""
+    from ppl.pmx_b200.torch_function.dynamic_batching import masked_attention as M
+    real, asked = M.lib, []
+
+    class Lib:
+        def __getattr__(self, name):
+            if name == "pmx_attention_workspace_bytes":
+                asked.append(name)
+            return getattr(real, name)
+    monkeypatch.setattr(M, "lib", Lib())
+    q = torch.ones(4, 2, 64, device="cuda", dtype=torch.float16)
+    k = torch.ones(4096, 2, 64, device="cuda", dtype=torch.float16)
+    for n in (1, 2):
+        DB.prompt_attention(q, k, k, i64([0, 4]).int(), i64([0, 4096]), 4, 4096, 2, 64)
+        assert len(asked) == n
