@@ -23,11 +23,11 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found; set NVCC or add it to PATH")
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(HOST):
+def _stale(target: str) -> bool:
+    if not os.path.exists(target):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(HOST))
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
+    t = os.path.getmtime(target)
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if target == LIB or f == "host_calls.cpp"]
     deps.append(os.path.join(PKG, "..", "..", "include", "pmx_moe.h"))
     return any(os.path.getmtime(d) > t for d in deps)
 
@@ -39,18 +39,37 @@ def _host_command() -> list:
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
     inc = [f"-I{d}" for d in (*cpp_extension.include_paths(), cuda, sysconfig.get_paths()["include"])]
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    built_for = f"torch {torch.__version__}, python {sys.version_info[0]}.{sys.version_info[1]}"
     return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            *inc, os.path.join(CSRC, "host_calls.cpp"), "-o", HOST, f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
-            "-ltorch_python"]
+            f'-DPMX_BUILT_FOR="{built_for}"', *inc, os.path.join(CSRC, "host_calls.cpp"), "-o", HOST + ".tmp", f"-L{lib}", "-lc10",
+            "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+
+
+def _build_host() -> None:
+    """The host calls need torch's and Python's headers.  The operators run without them, a few microseconds a call later:
+    a failure is reported and leaves none behind, and does not keep the library from being built."""
+    try:
+        done = subprocess.run(_host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        failure = f"exit status {done.returncode}\n{done.stdout}" if done.returncode else ""
+        if not done.returncode:
+            os.replace(HOST + ".tmp", HOST)
+    except Exception as e:
+        failure = f"{type(e).__name__}: {e}\n"
+    if failure:
+        sys.stderr.write(f"--- host_calls.cpp was not built\n{failure}\n")
+        if os.path.exists(HOST):
+            os.remove(HOST)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile every .cu of csrc/ into one shared library, and the host calls beside it; returns the library's path."""
-    if not force and not _stale():
+    if force or _stale(HOST):
+        _build_host()
+    if not force and not _stale(LIB):
         return LIB
     nvcc = _nvcc()
     objs = []
-    procs = [("host_calls.cpp", subprocess.Popen(_host_command(), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))]
+    procs = []
     for src in SOURCES:
         obj = os.path.join(CSRC, src[:-3] + ".o")
         cmd = [nvcc, *ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",

@@ -5,7 +5,8 @@
 // converting -- tensors on the current CUDA device, index arrays dense and 64 bits wide, views that the kernels
 // read in place, no gradient and no tangent asked for, no export under way -- and call the C ABI (include/pmx_moe.h).  For any other
 // call they return None, and the operators in torch_function/dynamic_batching check, convert and raise as they would
-// without this file.  A failed call comes back as its status.
+// without this file.  They do run without it: it is used where it was built for the torch and the Python at hand (built_for).
+// A failed call comes back as its status.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ATen.h>
@@ -356,4 +357,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_calls", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host_calls(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__host_calls(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", PMX_BUILT_FOR)) Py_CLEAR(m);
+  return m;
+}

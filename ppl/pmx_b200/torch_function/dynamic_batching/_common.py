@@ -3,24 +3,44 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import sys
+import warnings
 
 import torch
 from torch.autograd import forward_ad
 
 from ..._cabi import lib
 
-try:
-    from ... import _host_calls as host
-except ImportError as e:
-    raise ImportError("ppl/pmx_b200/_host_calls.so cannot be loaded: build it with `python -m ppl.pmx_b200.build`") from e
-host.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
-    "pmx_rotary_embedding", "pmx_prompt_attention", "pmx_tree_cache_attention", "pmx_compact_cache",
-    "pmx_attention_workspace_bytes")))
+
+class _GeneralPath:
+    """Stands in for the host calls: no call is a regular one."""
+    rotary = prompt = tree = compact = staticmethod(lambda *args: None)
+
+
+def _host_calls():
+    """The short way through the host (csrc/host_calls.cpp), where it was built for this torch and this Python.  It saves a call
+    a few microseconds; without it the operators check and convert in Python."""
+    try:
+        from ... import _host_calls as calls
+        built, here = calls.built_for, f"torch {torch.__version__}, python {sys.version_info[0]}.{sys.version_info[1]}"
+        if built != here:
+            raise ImportError(f"built for {built}, this is {here}")
+        calls.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in (
+            "pmx_rotary_embedding", "pmx_prompt_attention", "pmx_tree_cache_attention", "pmx_compact_cache",
+            "pmx_attention_workspace_bytes")))
+        return calls
+    except (ImportError, AttributeError) as e:
+        warnings.warn(f"ppl/pmx_b200/_host_calls.so is not used, which costs each call of the attention block a few microseconds "
+                      f"({e}); `python -m ppl.pmx_b200.build` builds it", RuntimeWarning)
+        return _GeneralPath
+
+
+host = _host_calls()
 
 _NULL = contextlib.nullcontext()
 # the raw stream handle and the current device without the objects that torch.cuda wraps them in: these
 # calls cost a few microseconds of host time in all, which is what a decode step's launches are bound by
-raw_stream = torch._C._cuda_getCurrentRawStream
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def on_device(index: int):

@@ -235,3 +235,19 @@ def test_workspace_is_asked_for_at_every_call(DB, monkeypatch):
     for n in (1, 2):
         DB.prompt_attention(q, k, k, i64([0, 4]).int(), i64([0, 4096]), 4, 4096, 2, 64)
         assert len(asked) == n
+
+
+def test_results_do_not_depend_on_the_way_through_the_host(DB, monkeypatch):
+    from ppl.pmx_b200.torch_function.dynamic_batching import _common, cache_rows, masked_attention, rotary
+    rng = np.random.default_rng(0)
+    t = [dev(values(rng, (5, 2, 64), "f16"), "f16") for _ in range(3)] + [dev(values(rng, (64,), "f16"), "f16")]
+    cache = dev(values(rng, (9, 1, 2, 2, 64), "f16"), "f16")
+
+    def results():
+        c = cache.clone()
+        return [x for call in every_operator(DB, *t, c, torch.int64).values() for r in [call()]
+                for x in (r if isinstance(r, tuple) else (r,))] + [c]
+    want = results()
+    for module in (cache_rows, masked_attention, rotary):
+        monkeypatch.setattr(module, "host", _common._GeneralPath)
+    assert all(torch.equal(a, b) for a, b in zip(results(), want))

@@ -1,7 +1,13 @@
 """The attention block's host side without a GPU: what asks for a derivative, what the package needs to be imported, what an
 export holds, sizes of workspaces."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -23,3 +29,48 @@ def test_gradients_and_tangents_are_noticed(DB):
         with torch.no_grad():
             assert wants_grad(dual)
     assert not wants_grad(dual)
+
+
+@pytest.mark.parametrize("calls", ["None", "types.SimpleNamespace(built_for='torch 1.0, python 3.1')", "types.SimpleNamespace()"])
+def test_the_package_does_without_the_host_calls(calls):
+    """Missing, not loadable, or of another torch: a warning, and every call takes the general path."""
+    code = f"""
+import sys, types, warnings
+sys.modules["ppl.pmx_b200._host_calls"] = {calls}
+with warnings.catch_warnings(record=True) as said:
+    warnings.simplefilter("always")
+    import ppl.pmx_b200.torch_function as F
+assert any("_host_calls.so is not used" in str(w.message) for w in said), said
+import torch
+DB = F.dynamic_batching
+q, i = torch.zeros(4, 2, 64), torch.arange(3)
+for call in (lambda: DB.rotary_position_embedding(q, q, i, i[:2]), lambda: DB.prompt_attention(q, q, q, i, i, 2, 2, 2, 64),
+             lambda: DB.tree_cache_attention(q, q, q, i, i[:2], i[:2], torch.zeros(4).long(), 2, 2, torch.zeros(8, 1, 2, 2, 64), 2, 64),
+             lambda: DB.compact_cache(torch.zeros(8, 1, 2, 2, 64), i[:2], i[:2], i, i[:2], 1)):
+    try:
+        call()
+        raise SystemExit("not refused")
+    except RuntimeError as e:
+        assert "no CPU fallback" in str(e)
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_the_host_calls_are_used_here(DB):
+    from ppl.pmx_b200 import _host_calls
+    from ppl.pmx_b200.torch_function.dynamic_batching import _common
+    assert _common.host is _host_calls
+
+
+def test_a_failed_build_of_the_host_calls_leaves_none(tmp_path, monkeypatch, capsys):
+    from ppl.pmx_b200 import build
+    target = tmp_path / "_host_calls.so"
+    target.write_bytes(b"of an earlier build")
+    monkeypatch.setattr(build, "HOST", str(target))
+    monkeypatch.setattr(build, "_host_command", lambda: ["false"])
+    build._build_host()
+    assert not target.exists()
+    monkeypatch.setattr(build, "_host_command", lambda: 1 / 0)
+    build._build_host()
+    assert capsys.readouterr().err.count("host_calls.cpp was not built") == 2
