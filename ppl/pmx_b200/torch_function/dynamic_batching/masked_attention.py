@@ -137,6 +137,11 @@ def _tree(query, current_key, current_value, seqstarts, cachestarts, start_pos, 
     return out
 
 
+def _length(g, n):
+    """A length of an exported call: an input of the node, a constant where the call has a number."""
+    return n if isinstance(n, torch._C.Value) else g.op("Constant", value_t=torch.tensor([int(n)]))
+
+
 class PromptAttention(torch.autograd.Function):
     """opmx.dynamic_batching::PromptAttention; no backward."""
 
@@ -144,7 +149,8 @@ class PromptAttention(torch.autograd.Function):
     def symbolic(g, query, key, value, seqstarts, kvstarts, max_seqlen, max_kvlen, num_heads: int, head_dim: int,
                  is_causal: bool = True, num_kv_heads: int = 0, scale=None, logit_cap: float = 0.0, alibi_slopes=None,
                  prefix_lens=None):
-        args = [query, key, value, seqstarts, kvstarts] + [t for t in (alibi_slopes, prefix_lens) if t is not None]
+        args = [query, key, value, seqstarts, kvstarts, _length(g, max_seqlen), _length(g, max_kvlen)]
+        args += [t for t in (alibi_slopes, prefix_lens) if t is not None]
         return g.op("opmx.dynamic_batching::PromptAttention", *args, num_heads_i=num_heads, head_dim_i=head_dim,
                     is_causal_i=is_causal, num_kv_heads_i=num_kv_heads, scale_f=scale or 1.0 / math.sqrt(head_dim),
                     logit_cap_f=logit_cap, alibi_slopes_i=alibi_slopes is not None,
@@ -165,7 +171,8 @@ class TreeCacheAttention(torch.autograd.Function):
                  max_kvlen, cache, num_heads: int, head_dim: int, num_kv_heads: int = 0, num_layer: int = 1,
                  layer_idx: int = 0, cache_layout: int = 0, scale=None, logit_cap: float = 0.0):
         return g.op("opmx.dynamic_batching::TreeCacheAttention", query, current_key, current_value, seqstarts,
-                    cachestarts, start_pos, tree_mask, cache, num_heads_i=num_heads, head_dim_i=head_dim,
+                    cachestarts, start_pos, tree_mask, _length(g, max_seqlen), _length(g, max_kvlen), cache,
+                    num_heads_i=num_heads, head_dim_i=head_dim,
                     num_kv_heads_i=num_kv_heads, num_layer_i=num_layer, layer_idx_i=layer_idx,
                     cache_layout_i=cache_layout, scale_f=scale or 1.0 / math.sqrt(head_dim),
                     logit_cap_f=logit_cap).setTypeAs(query)

@@ -74,3 +74,30 @@ def test_a_failed_build_of_the_host_calls_leaves_none(tmp_path, monkeypatch, cap
     monkeypatch.setattr(build, "_host_command", lambda: 1 / 0)
     build._build_host()
     assert capsys.readouterr().err.count("host_calls.cpp was not built") == 2
+
+
+def test_exported_attention_keeps_its_lengths(DB):
+    """max_seqlen (rows behind it are zero) and max_kvlen are inputs of the nodes, given as ints or as tensors."""
+    from torch.onnx._internal.torchscript_exporter import utils as U, _globals
+
+    class Block(torch.nn.Module):
+        def forward(s, q, k, starts, past, mask, cache, most):
+            a = DB.prompt_attention(q, k, k, starts, starts, 3, most, 4, 64, num_kv_heads=2, alibi_slopes=torch.ones(4))
+            return DB.tree_cache_attention(a, k, k, starts, past, past, mask, most, 7, cache, 4, 64, num_kv_heads=2)
+
+    z = torch.zeros
+    args = (z(4, 4, 64), z(4, 2, 64), torch.tensor([0, 4]), z(1, dtype=torch.int64), torch.ones(4, dtype=torch.int64),
+            z(9, 1, 2, 2, 64), torch.tensor([5]))
+    _globals.GLOBALS.export_onnx_opset_version = 11
+    _globals.GLOBALS.in_onnx_export = True
+    try:
+        with U.exporter_context(Block(), torch.onnx.TrainingMode.EVAL, False):
+            graph, _, _ = U._model_to_graph(Block(), args, do_constant_folding=False)
+    finally:
+        _globals.GLOBALS.in_onnx_export = False
+    prompt, tree = [n for n in graph.nodes() if n.kind().startswith("opmx")]
+    most = list(graph.inputs())[6]
+    constant = lambda v: v.node().t("value").tolist()        # noqa: E731
+    p, t = list(prompt.inputs()), list(tree.inputs())
+    assert len(p) == 8 and constant(p[5]) == [3] and p[6].debugName() == most.debugName() and prompt.i("alibi_slopes") == 1
+    assert len(t) == 10 and t[7].debugName() == most.debugName() and constant(t[8]) == [7]
