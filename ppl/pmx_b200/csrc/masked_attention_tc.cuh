@@ -24,8 +24,8 @@
 // The bound is the tensor pipe and, next to it, the exponentials: per 128 x 128 scores 1024 cycles of products (head
 // size 128) against 1024 of the special function unit, and a tile's softmax lies between its own two products.  So a
 // half's softmax runs beside the other half's products, and is kept short.  The running maximum moves only when a
-// row's new maximum lies more than 2^8 above it, so that O in tensor memory is rescaled rarely; probabilities stay below
-// 2^8, exact in the 16-bit types' range, and the sum divides the same scale out again.
+// row's new maximum lies more than 2^8 above it (2^4 in f16), so that O in tensor memory is rescaled rarely; probabilities
+// stay below 2^8 (2^15 in f16, scaled up by 2^11), and the sum divides the same scale out again.
 //
 // A masked score becomes -inf whatever the product holds.  A masked VALUE needs more: 0 * inf and 0 * NaN are NaN in
 // the second product, so in the tiles that are not seen whole by every row, values that are not finite are replaced by
@@ -39,7 +39,12 @@ constexpr int kQueue = 4;                   // items under way
 constexpr int kMinTiles = 4;                // key tiles that a split of a pair of row tiles should have at least,
 constexpr int kFlatTiles = 2;               // and that a CTA should have of the list of all key tiles (2: one for each half;
                                             // two drafted trees over 700 rows: a tenth faster than with 4)
-constexpr float kLazy = 8.0f;               // log2 of how far a maximum may run ahead
+// How far (log2) a row's maximum may run ahead of the one in use, and the power of two that probabilities are scaled by, in
+// product and sum alike.  In f16, which ends at 2^16 and below at 2^-24, a weak key's probability would be lost in the product and
+// stay in the sum: scaled, it is exact to half a step down to 2^-25 of the strongest key's and lost below 2^-36.  bf16 has
+// the range of 32 bits.
+template <typename T> constexpr float kLazy = std::is_same<T, __half>::value ? 4.0f : 8.0f;
+template <typename T> constexpr float kScaleUp = std::is_same<T, __half>::value ? 11.0f : 0.0f;
 constexpr unsigned long long kAttnWaitNs = 2000000000ull;
 
 __device__ int g_attention_status[4];       // record of a bounded wait that ran out: code, role, tile, CTA
@@ -1059,7 +1064,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         if (i == 0) {
           m = mx;
         } else {
-          const bool moves = !(mx <= m + kLazy) && !(m == INFINITY);
+          const bool moves = !(mx <= m + kLazy<T>) && !(m == INFINITY);
           if (__any_sync(0xFFFFFFFFu, moves)) {
             const float f = moves && m != mx ? ex2(m - mx) : 1.0f;
             m = moves ? mx : m;
@@ -1076,7 +1081,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
           }
         }
         // -inf: nothing seen so far; +inf: inf - inf, NaN for the whole row
-        const float base = m == -INFINITY ? 0.f : (m == INFINITY ? __int_as_float(0x7FC00000) : m);
+        const float base = m == -INFINITY ? 0.f : (m == INFINITY ? __int_as_float(0x7FC00000) : m - kScaleUp<T>);
         f32x2 sum = pair2(0.f, 0.f), sum1 = sum;
         auto probabilities = [&](int c) {      // exponentials and sum of 32 scores, and their probabilities into tensor memory
           const f32x2 nb = pair2(-base, -base), sc = pair2(sl, sl);

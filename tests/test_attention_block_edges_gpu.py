@@ -7,7 +7,7 @@ import torch
 
 from oracle import attention_block as ab
 from tests.helpers import TORCH_DT, dev, host
-from tests.test_attention_block_gpu import DB, cache_of, check_attention, i64, no_wait_ran_out, prompt_case, values  # noqa: F401
+from tests.test_attention_block_gpu import DB, UNIT, cache_of, check_attention, i64, no_wait_ran_out, prompt_case, values  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -251,3 +251,27 @@ def test_results_do_not_depend_on_the_way_through_the_host(DB, monkeypatch):
     for module in (cache_rows, masked_attention, rotary):
         monkeypatch.setattr(module, "host", _common._GeneralPath)
     assert all(torch.equal(a, b) for a, b in zip(results(), want))
+
+
+# ------------------------------------------------------------------------------- weak keys in f16
+@pytest.mark.parametrize("log2", [17.25, 25.5, 30.75])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_many_weak_keys_beside_a_dominant_one(DB, log2, first, dtype):
+    """n keys of probability 2^-log2 beside one of (nearly) 1, whose value is zero: together they are the result.
+    On the way a probability takes 16 bits, scaled by 2^11 in f16: half a step of 2^-11 of it, or 2^-25 of the scaled value
+    where that is below 2^-14: 2^-36 absolute."""
+    T, H, D, n = 2560, 8, 64, 60000
+    rng = np.random.default_rng(1)
+    q = torch.zeros(T, H, D, device="cuda", dtype=TORCH_DT[dtype])
+    k = torch.zeros(n + 1, H, D, device="cuda", dtype=TORCH_DT[dtype])
+    v = torch.ones(n + 1, H, D, device="cuda", dtype=TORCH_DT[dtype])
+    at = 0 if first else n
+    q[..., 0], k[at, :, 0], v[at] = 4.0, log2 * math.log(2) / 4, 0.0
+    s = 4.0 * float(k[at, 0, 0])
+    w = n * math.exp(-s)
+    want = w / (1 + w)
+    got = DB.prompt_attention(q, k, v, i64([0, T]), i64([0, n + 1]), T, n + 1, H, D, is_causal=False, scale=1.0)
+    # two roundings to 16 bits; the products' sum over n / 16 steps and the probabilities' in 32; scores of 2^-19
+    tol = (2 * UNIT[dtype] + (n / 8 + n / 128) * 2.0 ** -24 + 2.0 ** -19) * want + n * 2.0 ** -36 * (dtype == "f16") + 2.0 ** -25
+    assert (got.double() - want).abs().max() <= tol
