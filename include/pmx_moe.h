@@ -437,7 +437,8 @@ int pmx_prompt_attention(const pmx_prompt_attention_args* args, void* stream);
  * tokens; their keys and values are stored at cache rows cachestarts[b] + start_pos[b] + i, and token i sees the
  * start_pos[b] cached rows and the drafted tokens j of its sequence with bit j of tree_mask[token] set (its own
  * bit included, if it is to see itself).  Scores, empty rows, types and kernels as for pmx_prompt_attention;
- * cache strides as for pmx_decode_cache_attention, cache_rows rows in all (new rows outside are not stored).
+ * cache strides as for pmx_decode_cache_attention, cache_rows rows in all.  Rows outside the cache are neither
+ * seen nor stored, nor are new rows stored in front of cachestarts[b] (a negative start_pos).
  */
 typedef struct pmx_tree_attention_args {
   const void *query, *current_key, *current_value;

@@ -52,6 +52,7 @@ struct Sequence {
   int n;           // queries
   int64_t kv0;     // first row of `past`
   int64_t len;     // keys in `past`
+  int64_t store;   // trees: row of `past` that takes the first drafted token's key and value; see stored()
   int64_t shift;   // position of query i among the keys: i + shift
   int64_t prefix;  // keys below it are seen by all queries (0: none)
 };
@@ -64,17 +65,29 @@ __device__ __forceinline__ Sequence load_sequence(const AttnArgs& a, int b) {
   const int64_t q1 = clamp64(__ldcg(a.seqstarts + b + 1), s.q0, a.Tq);
   s.n = (int)(q1 - s.q0 < a.max_seqlen ? q1 - s.q0 : a.max_seqlen);
   if (a.tree_mask) {
-    s.kv0 = clamp64(__ldcg(a.cachestarts + b), 0, a.past.rows);
-    s.len = clamp64(__ldcg(a.start_pos + b), 0, a.past.rows - s.kv0);
+    // of rows [c, c + p) those that exist; 2^40 is beyond any cache and keeps the sums small
+    constexpr int64_t kFar = 1ll << 40;
+    const int64_t c = clamp64(__ldcg(a.cachestarts + b), -kFar, kFar);
+    s.store = c + clamp64(__ldcg(a.start_pos + b), -kFar, kFar);
+    s.kv0 = clamp64(c, 0, a.past.rows);
+    s.len = clamp64(s.store, s.kv0, a.past.rows) - s.kv0;
     s.shift = 0;
     s.prefix = 0;
   } else {
     s.kv0 = clamp64(__ldcg(a.kvstarts + b), 0, a.past.rows);
     s.len = clamp64(__ldcg(a.kvstarts + b + 1), s.kv0, a.past.rows) - s.kv0;
+    s.store = 0;
     s.shift = s.len - (q1 - s.q0);
     s.prefix = a.prefix ? clamp64(__ldcg(a.prefix + b), 0, s.len) : 0;
   }
   return s;
+}
+
+// The row that takes drafted token i's key and value, or -1: rows outside the cache are dropped, and so are those in front of
+// their sequence's first (a negative start_pos), which are another's.
+__device__ __forceinline__ int64_t stored(const AttnArgs& a, const Sequence& s, int64_t i) {
+  const int64_t row = s.store + i;
+  return row >= s.kv0 && row < a.past.rows ? row : -1;
 }
 
 // keys of `past` that query i sees: the first this many
@@ -114,8 +127,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) attention_row_kernel(const __g
   for (int d = lane; d < a.D; d += 32) sq[warp][d] = Elem<T>::to_f(q[d]);
   __syncwarp();
   if (a.tree_mask && h % (a.Hq / a.Hkv) == 0) {    // one head of each group stores the new key and value
-    const int64_t row = s.kv0 + s.len + i;
-    if (row < a.past.rows) {
+    const int64_t row = stored(a, s, i);
+    if (row >= 0) {
       const T* kc = reinterpret_cast<const T*>(a.cur.k) + t * a.cur.k_row + (int64_t)hk * a.cur.k_head;
       const T* vc = reinterpret_cast<const T*>(a.cur.v) + t * a.cur.v_row + (int64_t)hk * a.cur.v_head;
       T* kd = reinterpret_cast<T*>(const_cast<void*>(a.past.k)) + row * a.past.k_row + (int64_t)hk * a.past.k_head;

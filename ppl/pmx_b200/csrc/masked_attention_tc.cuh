@@ -787,7 +787,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
         int64_t end = ta;                             // the first token that needs a look-up
         Sequence s;
         s.n = 0;
-        s.q0 = s.kv0 = s.len = 0;
+        s.q0 = s.kv0 = s.len = s.store = 0;
         for (int64_t t = ta; t < tb; ++t) {
           if (t >= end) {
             int before = 0;
@@ -800,8 +800,8 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
               if (t < s.q0 + s.n) end = s.q0 + s.n;
             }
           }
-          const int64_t row = s.kv0 + s.len + (t - s.q0);
-          if (t - s.q0 < 0 || t - s.q0 >= s.n || row >= a.past.rows) continue;
+          const int64_t row = stored(a, s, t - s.q0);
+          if (t - s.q0 < 0 || t - s.q0 >= s.n || row < 0) continue;
           for (int i0 = lane; i0 < count; i0 += 32 * 4) {
             uint4 held[4];
             T* dst[4];

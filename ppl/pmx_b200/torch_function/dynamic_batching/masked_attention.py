@@ -222,7 +222,8 @@ def tree_cache_attention(query: torch.Tensor, current_key: torch.Tensor, current
     Sequence b brings the tokens seqstarts[b]..seqstarts[b+1], at most 64.  Token i of it sees the start_pos[b] cached
     rows from cachestarts[b] on, and drafted token j of its sequence where bit j of tree_mask[token] is set (int64
     [tokens]; a token that is to see itself needs its own bit).  The new keys and values are stored into `cache`, in place,
-    at rows cachestarts[b] + start_pos[b] + i (rows outside the cache are dropped); compact_cache() then moves the accepted
+    at rows cachestarts[b] + start_pos[b] + i (rows outside the cache are neither seen nor stored, nor are rows stored in
+    front of cachestarts[b], where a negative start_pos leads); compact_cache() then moves the accepted
     ones together.  max_seqlen: at least the most drafted tokens of a sequence, max_kvlen: at least the most cached plus
     drafted rows.  Cache layouts 0..3 as multi_head_cache_attention(); scores, types and empty rows as
     prompt_attention()."""

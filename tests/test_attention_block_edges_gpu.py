@@ -7,7 +7,7 @@ import torch
 
 from oracle import attention_block as ab
 from tests.helpers import TORCH_DT, dev, host
-from tests.test_attention_block_gpu import DB, UNIT, cache_of, check_attention, i64, no_wait_ran_out, prompt_case, values  # noqa: F401
+from tests.test_attention_block_gpu import DB, UNIT, cache_of, check_attention, i64, no_wait_ran_out, prompt_case, starts, values  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -275,3 +275,32 @@ def test_many_weak_keys_beside_a_dominant_one(DB, log2, first, dtype):
     # two roundings to 16 bits; the products' sum over n / 16 steps and the probabilities' in 32; scores of 2^-19
     tol = (2 * UNIT[dtype] + (n / 8 + n / 128) * 2.0 ** -24 + 2.0 ** -19) * want + n * 2.0 ** -36 * (dtype == "f16") + 2.0 ** -25
     assert (got.double() - want).abs().max() <= tol
+
+
+# ------------------------------------------------------------------------------- rows outside the cache
+@pytest.mark.parametrize("dtype,D", [("f16", 64), ("f32", 48)])
+def test_drafted_rows_outside_the_cache_or_before_their_sequence_are_dropped(DB, dtype, D):
+    """A sequence that begins before the cache stores and sees only the rows that exist; one with a negative start_pos sees no
+    row and stores none in front of its first."""
+    rng = np.random.default_rng(3)
+    Hq, Hkv, rows = 4, 2, 60
+    cache_np = cache_of(rng, 2, rows, 1, Hkv, D, dtype)
+    n = [4, 4, 3, 2, 2]
+    cs, sp = [-4, 20, 50, 1 << 62, -(1 << 62)], [3, -2, 12, 1 << 62, -(1 << 62)]
+    ss, T = starts(n), sum(n)
+    q, k, v = (values(rng, (T, h, D), dtype) for h in (Hq, Hkv, Hkv))
+    masks = np.array([(1 << (i + 1)) - 1 for m in n for i in range(m)], np.int64)
+    cache = dev(cache_np, dtype)
+    got = DB.tree_cache_attention(dev(q, dtype), dev(k, dtype), dev(v, dtype), i64(ss), i64(cs), i64(sp), i64(masks), 4, 20, cache,
+                                  Hq, D, num_kv_heads=Hkv, cache_layout=2)
+    want = cache_np.copy()
+    for b, m in enumerate(n):
+        for i in range(m):
+            row = cs[b] + sp[b] + i
+            if max(cs[b], 0) <= row < rows:
+                want[0, 0, row], want[0, 1, row] = k[ss[b] + i], v[ss[b] + i]
+    assert np.array_equal(host(cache), want)
+    lo = [0, 20, 50, 0, 0]
+    past = [0, 0, 10, 0, 0]
+    ref = ab.tree_attention(q, k, v, cache_np.copy(), 2, 0, ss, lo, past, masks, 1 / math.sqrt(D))
+    check_attention(got, ref, dtype, D, 20, 0.0, dtype != "f32")
