@@ -121,8 +121,10 @@ def _tree(query, current_key, current_value, seqstarts, cachestarts, start_pos, 
     tree_mask = index(name, "tree_mask", tree_mask, Tq)
     max_seqlen, max_kvlen = host_int(name, "max_seqlen", max_seqlen), host_int(name, "max_kvlen", max_kvlen)
     out = q.new_empty((Tq, num_heads, head_dim))
-    if Tq == 0 or rows == 0:
-        return out.zero_()
+    if Tq == 0:
+        return out
+    if rows == 0:
+        raise ValueError(f"{name}: the cache has no rows")
     q0, q1, _ = q.stride()
     k0, k1, _ = k.stride()
     v0, v1, _ = v.stride()

@@ -304,3 +304,10 @@ def test_drafted_rows_outside_the_cache_or_before_their_sequence_are_dropped(DB,
     past = [0, 0, 10, 0, 0]
     ref = ab.tree_attention(q, k, v, cache_np.copy(), 2, 0, ss, lo, past, masks, 1 / math.sqrt(D))
     check_attention(got, ref, dtype, D, 20, 0.0, dtype != "f32")
+
+
+def test_a_cache_without_rows_is_refused(DB):
+    q = torch.ones(2, 2, 64, device="cuda", dtype=torch.float16)
+    cache = torch.empty(0, 1, 2, 2, 64, device="cuda", dtype=torch.float16)
+    with pytest.raises(ValueError, match="rows"):
+        DB.tree_cache_attention(q, q, q, i64([0, 2]), i64([0]), i64([0]), i64([1, 3]), 2, 2, cache, 2, 64)
