@@ -462,7 +462,7 @@ int pmx_attention_check(int32_t out[4], void* stream);
  * accept_starts[b+1] - accept_starts[b] (at most max_accept <= 64), in every layer, keys and values:
  *   cache row base + i <- cache row base + accept_index[accept_starts[b] + i],  base = cachestarts[b] + start_pos[b],
  * all rows of a sequence read before any is written, so the indices may come in any order and repeat.  A
- * negative index, and a row outside the cache_rows rows, is skipped.  index_count: entries of accept_index.  The
+ * negative index, and a row outside the cache_rows rows or in front of cachestarts[b], is skipped.  index_count: entries of accept_index.  The
  * cache element (row, layer, kv, head, d) lies at row*row_stride + layer*layer_stride + kv*kv_stride +
  * head*head_stride + d.
  */

@@ -37,13 +37,14 @@ __global__ void __launch_bounds__(kWarps * 32) compact_cache_kernel(const __grid
   const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) {
     const int64_t first = __ldcg(a.accept_starts + b), last = __ldcg(a.accept_starts + b + 1);
-    const int64_t base = __ldcg(a.cachestarts + b) + __ldcg(a.start_pos + b);
+    const int64_t start = __ldcg(a.cachestarts + b), base = start + __ldcg(a.start_pos + b);
+    const int64_t lowest = start > 0 ? start : 0;        // rows in front of it are another sequence's, or none
     const int64_t n = first < 0 || last > a.index_count ? 0 : (last - first < a.max_accept ? last - first : a.max_accept);
     int before = 0;
     for (int i = lane; i < kMaxAccept; i += 32) {
       const int64_t from = i < n ? __ldcg(a.accept_index + first + i) : -1;
-      // a row that stays, or one outside the cache, is left alone
-      const bool on = from >= 0 && from != i && base + from >= 0 && base + from < a.rows && base + i >= 0 && base + i < a.rows;
+      // a row that stays, or one outside the cache or the sequence, is left alone
+      const bool on = from >= 0 && from != i && base + from >= lowest && base + from < a.rows && base + i >= lowest && base + i < a.rows;
       const unsigned some = __ballot_sync(0xFFFFFFFFu, on);
       if (on) {
         const int at = before + __popc(some & ((1u << lane) - 1));

@@ -12,10 +12,11 @@ def compact_cache(cache: torch.Tensor, cachestarts: torch.Tensor, start_pos: tor
     """Keeps, of the rows that tree_cache_attention() stored, those of the accepted tokens -> `cache`, changed in place.
 
     Sequence b accepts the drafted tokens accept_index[accept_starts[b]..accept_starts[b+1]] (their places in the draft,
-    at most max_accept <= 64, what is listed behind them is left out; normally a path from the root): row base + i takes the row base + accept_index[..i], with
-    base = cachestarts[b] + start_pos[b], in all layers, keys and values.  All rows of a sequence are read before one is
-    written, so the indices may come in any order and repeat; a negative index leaves its row alone.  The caller's next
-    start_pos is start_pos + the number accepted.  Rows of different sequences must not overlap."""
+    at most max_accept <= 64: entries behind those are left out; normally a path from the root): row base + i takes the row
+    base + accept_index[..i], with base = cachestarts[b] + start_pos[b], in all layers, keys and values.  All rows of a
+    sequence are read before one is written, so the indices may come in any order and repeat; a negative index leaves its
+    row alone, and so does one that leads outside the cache or in front of cachestarts[b].  The caller's next start_pos is
+    start_pos + the number accepted.  Rows of different sequences must not overlap."""
     status = host.compact(cache, cachestarts, start_pos, accept_starts, accept_index, max_accept, num_layer, cache_layout)
     if status is not None:           # None: not the regular case
         check(status)

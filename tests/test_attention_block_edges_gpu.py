@@ -180,6 +180,22 @@ def test_compaction_moves_no_more_than_max_accept(DB, most, listed):
     assert np.array_equal(host(t), cache)
 
 
+def test_compaction_stays_within_its_sequence(DB):
+    """A negative start_pos, or a sequence in front of the cache: no row of another sequence moves or is taken."""
+    rng = np.random.default_rng(4)
+    cache = cache_of(rng, 0, 40, 1, 2, 16, "f16")
+    t = dev(cache, "f16")
+    cs, sp = [10, -6, 20, (1 << 63) - 1], [-3, 5, 4, (1 << 63) - 1]
+    picks = [[1, 2, 5, 6, 4], [3, 4, 2, 0], [2, 0], [4, 5, 6]]
+    DB.compact_cache(t, i64(cs), i64(sp), i64(starts([len(p) for p in picks])), i64(sum(picks, [])), 5)
+    want = cache.copy()
+    for c, s, p in zip(cs, sp, picks):
+        for i, j in enumerate(p):
+            if max(c, 0) <= c + s + i < 40 and max(c, 0) <= c + s + j < 40:
+                want[c + s + i] = cache[c + s + j]
+    assert np.array_equal(host(t), want)
+
+
 # ------------------------------------------------------------------------------- tangents, memory, workspaces
 def every_operator(DB, q, k, v, w, cache, indices):
     ss, z = i64([0, 5]).to(indices), i64([0])
