@@ -1292,7 +1292,9 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
     const int64_t i = t - __reduce_max_sync(0xFFFFFFFFu, start);
     if (b < 0 || b >= a.B || i >= a.max_seqlen) return;
     who = __ldcg(p.pieces + (int64_t)b * a.Hkv + h);
-    if (who.x == who.y) return;                    // in one piece: the result is there
+    // In one piece: the result is there.  Starts that do not rise can lead to a sequence without an item, whose entry was
+    // never written.
+    if (who.x < 0 || who.x >= who.y || who.y >= p.ctas) return;
     r = (int)i * p.group + head % p.group;
   }
   const int n = who.y - who.x + 1;                 // pieces, of which this warp takes every WARPS-th

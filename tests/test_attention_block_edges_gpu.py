@@ -293,6 +293,23 @@ def test_many_weak_keys_beside_a_dominant_one(DB, log2, first, dtype):
     assert (got.double() - want).abs().max() <= tol
 
 
+@pytest.mark.parametrize("fill", [0x7F, 0xFF, 0x01])
+def test_starts_that_do_not_rise_stay_inside(DB, fill):
+    """Sequences that overlap or end before they begin, over keys in many pieces: what is computed then is of no use, but
+    nothing outside the tensors is touched, whatever the workspace held before."""
+    Hq, Hkv, D = 4, 2, 64
+    q = torch.ones(8, Hq, D, device="cuda", dtype=torch.float16)
+    k = torch.ones(9100, Hkv, D, device="cuda", dtype=torch.float16)
+    cache = torch.ones(9200, 1, 2, Hkv, D, device="cuda", dtype=torch.float16)
+    for ss in ([0, 4, 2, 6], [7, 3, 5, 1], [0, -4, 90, 8], [3, 3, 1, 1]):
+        junk = [torch.full((n,), fill, device="cuda", dtype=torch.uint8) for n in (1 << 20, 8 << 20, 32 << 20)]
+        del junk
+        DB.prompt_attention(q, k, k, i64(ss), i64([0, 3000, 6000, 9100]), 4, 9100, Hq, D, num_kv_heads=Hkv)
+        DB.tree_cache_attention(q, k[:8], k[:8], i64(ss), i64([0, 3000, 6000]), i64([2900, 2900, 3100]), i64([-1] * 8), 4, 3110, cache,
+                                Hq, D, num_kv_heads=Hkv)
+    torch.cuda.synchronize()
+
+
 # ------------------------------------------------------------------------------- rows outside the cache
 @pytest.mark.parametrize("dtype,D", [("f16", 64), ("f32", 48)])
 def test_drafted_rows_outside_the_cache_or_before_their_sequence_are_dropped(DB, dtype, D):
