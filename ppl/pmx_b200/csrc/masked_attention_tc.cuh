@@ -1368,6 +1368,7 @@ TcPlan plan_tc(int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_
     return pl;
   if (Tq <= 0 || B <= 0 || Hq <= 0 || D <= 0 || max_seqlen <= 0 || max_kvlen <= 0 || Tq >= (1ll << 31)) return pl;
   if (max_seqlen > Tq) max_seqlen = Tq;
+  if (max_kvlen > (1ll << 31)) max_kvlen = 1ll << 31;      // more rows than tensors have here; products below stay in range
   pl.group = (int)(Hq / Hkv);
   pl.tokens = kTile / pl.group;
   pl.pair = max_seqlen > pl.tokens;

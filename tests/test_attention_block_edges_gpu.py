@@ -310,6 +310,18 @@ def test_starts_that_do_not_rise_stay_inside(DB, fill):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("lens", [[(3, 40), (1, 700)], [(300, 300), (2, 900)]])
+@pytest.mark.parametrize("most", [1 << 31, 1 << 57, (1 << 63) - 1])
+def test_lengths_without_a_bound(DB, lens, most):
+    """max_seqlen and max_kvlen are bounds; one that says nothing is as good as any."""
+    rng = np.random.default_rng(7)
+    q, k, v, ss, ks, ms, mk = prompt_case(rng, lens, 4, 2, 64, "bf16")
+    ref = ab.prompt_attention(q, k, v, ss, ks, True, 1 / 8.0)
+    for a, b in ((ms, most), (most, mk), (most, most)):
+        got = DB.prompt_attention(dev(q, "bf16"), dev(k, "bf16"), dev(v, "bf16"), i64(ss), i64(ks), a, b, 4, 64, num_kv_heads=2)
+        check_attention(got, ref, "bf16", 64, mk, 0.0)
+
+
 # ------------------------------------------------------------------------------- rows outside the cache
 @pytest.mark.parametrize("dtype,D", [("f16", 64), ("f32", 48)])
 def test_drafted_rows_outside_the_cache_or_before_their_sequence_are_dropped(DB, dtype, D):

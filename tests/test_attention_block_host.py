@@ -101,3 +101,15 @@ def test_exported_attention_keeps_its_lengths(DB):
     p, t = list(prompt.inputs()), list(tree.inputs())
     assert len(p) == 8 and constant(p[5]) == [3] and p[6].debugName() == most.debugName() and prompt.i("alibi_slopes") == 1
     assert len(t) == 10 and t[7].debugName() == most.debugName() and constant(t[8]) == [7]
+
+
+@pytest.mark.parametrize("tokens,sequences,heads,kv_heads,most", [(4, 1, 4, 2, 4), (64, 64, 64, 64, 1), (400, 1, 4, 2, 400),
+                                                                  (5000, 100, 8, 8, 300), (6400, 6400, 8, 8, 1)])
+def test_a_bound_on_the_keys_may_be_any_number(tokens, sequences, heads, kv_heads, most):
+    """max_kvlen is a bound: one beyond every tensor (no bound at all) plans what the largest possible one does."""
+    from ppl.pmx_b200._cabi import lib
+    size = lambda n: lib.pmx_attention_workspace_bytes(tokens, sequences, heads, kv_heads, 64, most, n, 0)     # noqa: E731
+    want = size(1 << 31)
+    assert 0 < want < 1 << 30 or want == 0 and most > 128
+    for n in ((1 << 31) + 1, 1 << 40, 1 << 57, 1 << 62, (1 << 63) - 1):
+        assert size(n) == want
