@@ -875,7 +875,8 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t s_tmem = tmem + lanes + half * 128, o_tmem = tmem + lanes + 256 + half * 128;
     constexpr float kLog2e = 1.4426950408889634f;
-    const float cap2 = a.cap * kLog2e, to_y = a.cap > 0.f ? a.scale / a.cap : 0.f;      // cap in log2 domain; s / c of a product
+    // cap in log2 domain; s / c of a product, finite so that a score of zero stays zero with a cap of next to nothing
+    const float cap2 = a.cap * kLog2e, to_y = a.cap > 0.f ? fminf(a.scale / a.cap, 1e30f) : 0.f;
     const float sl2 = a.scale * kLog2e;
     const bool score = a.cap > 0.f || a.slopes;       // scores are rewritten, in log2 domain then
     const float sl = score ? 1.0f : sl2;

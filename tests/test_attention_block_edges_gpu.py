@@ -269,6 +269,18 @@ def test_results_do_not_depend_on_the_way_through_the_host(DB, monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(results(), want))
 
 
+@pytest.mark.parametrize("cap", [1e-3, 1e-30, 1e-38, 1e-41, 1e30])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_caps_from_nothing_to_no_cap(DB, cap, dtype):
+    """Any positive cap: scores of zero among others stay zero, a cap near nothing leaves all keys alike."""
+    rng = np.random.default_rng(2)
+    q, k, v, ss, ks, ms, mk = prompt_case(rng, [(40, 140), (3, 9)], 2, 1, 64, dtype)
+    q[1], k[3] = 0, 0
+    got = DB.prompt_attention(dev(q, dtype), dev(k, dtype), dev(v, dtype), i64(ss), i64(ks), ms, mk, 2, 64, num_kv_heads=1,
+                              logit_cap=cap)
+    check_attention(got, ab.prompt_attention(q, k, v, ss, ks, True, 1 / 8.0, cap), dtype, 64, mk, min(cap, 30.0), dtype != "f32")
+
+
 # ------------------------------------------------------------------------------- weak keys in f16
 @pytest.mark.parametrize("log2", [17.25, 25.5, 30.75])
 @pytest.mark.parametrize("first", [True, False])
