@@ -6,6 +6,7 @@ import os
 import shutil
 import subprocess
 import sys
+import threading
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -32,6 +33,22 @@ def _stale(target: str) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _built_for() -> str:
+    """What the host calls are built for; the package uses them where it is the same."""
+    import torch
+    return f"torch {torch.__version__}, python {sys.version_info[0]}.{sys.version_info[1]}"
+
+
+def _host_stale() -> bool:
+    if _stale(HOST):
+        return True
+    try:
+        with open(HOST, "rb") as f:
+            return _built_for().encode() + b"\0" not in f.read()
+    except ImportError:                      # no torch: the build says so
+        return True
+
+
 def _host_command() -> list:
     import sysconfig
     import torch
@@ -39,9 +56,8 @@ def _host_command() -> list:
     cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
     inc = [f"-I{d}" for d in (*cpp_extension.include_paths(), cuda, sysconfig.get_paths()["include"])]
     lib = os.path.join(os.path.dirname(torch.__file__), "lib")
-    built_for = f"torch {torch.__version__}, python {sys.version_info[0]}.{sys.version_info[1]}"
     return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            f'-DPMX_BUILT_FOR="{built_for}"', *inc, os.path.join(CSRC, "host_calls.cpp"), "-o", HOST + ".tmp", f"-L{lib}", "-lc10",
+            f'-DPMX_BUILT_FOR="{_built_for()}"', *inc, os.path.join(CSRC, "host_calls.cpp"), "-o", HOST + ".tmp", f"-L{lib}", "-lc10",
             "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
 
 
@@ -63,10 +79,17 @@ def _build_host() -> None:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile every .cu of csrc/ into one shared library, and the host calls beside it; returns the library's path."""
-    if force or _stale(HOST):
-        _build_host()
-    if not force and not _stale(LIB):
-        return LIB
+    host = threading.Thread(target=_build_host)
+    if force or _host_stale():
+        host.start()
+    try:
+        return _build_library(verbose) if force or _stale(LIB) else LIB
+    finally:
+        if host.ident is not None:
+            host.join()
+
+
+def _build_library(verbose: bool) -> str:
     nvcc = _nvcc()
     objs = []
     procs = []

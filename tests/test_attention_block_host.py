@@ -76,6 +76,15 @@ def test_a_failed_build_of_the_host_calls_leaves_none(tmp_path, monkeypatch, cap
     assert capsys.readouterr().err.count("host_calls.cpp was not built") == 2
 
 
+def test_host_calls_of_another_torch_are_built_anew(monkeypatch):
+    from ppl.pmx_b200 import build
+    monkeypatch.setattr(build, "_stale", lambda target: False)
+    now = build._built_for()
+    assert not build._host_stale()
+    monkeypatch.setattr(build, "_built_for", lambda: now[:-1])
+    assert build._host_stale()
+
+
 def test_exported_attention_keeps_its_lengths(DB):
     """max_seqlen (rows behind it are zero) and max_kvlen are inputs of the nodes, given as ints or as tensors."""
     from torch.onnx._internal.torchscript_exporter import utils as U, _globals
