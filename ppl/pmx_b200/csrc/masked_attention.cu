@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "packed_f32.cuh"
 
 namespace pmx {
 namespace {

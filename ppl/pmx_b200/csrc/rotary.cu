@@ -17,6 +17,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "packed_f32.cuh"
 
 namespace pmx {
 namespace {
@@ -81,33 +82,14 @@ __device__ __forceinline__ void fill_table(const RotaryArgs& a, int64_t p, float
   __syncwarp();
 }
 
-// one spelling for both kernels, so that a value does not depend on which of them takes the call
+// Spelt as in the vector kernel: without a norm a value's bits do not depend on which of the two takes the call.  (With one they
+// may, by roundings in 32 bits: the vector kernel multiplies the weights into the coefficients.)
 __device__ __forceinline__ void rotate_pair(float& l, float& r, float c, float s) {
   const float x = l, y = r;
   l = fmaf(x, c, -(y * s));
   r = fmaf(y, c, x * s);
 }
 
-// ---- two 32-bit values per instruction
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pair2(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpair2(f32x2 v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // a 16-byte vector as V/2 pairs, and back with one rounding each
 template <typename T>
 __device__ __forceinline__ void unpack_pairs(const uint4& v, f32x2 (&x)[kVec<T> / 2]) {
