@@ -19,13 +19,16 @@
 // leaves in pieces is merged by a second kernel (fp32 results with maximum and sum).  Pairs with so few CTAs that SMs
 // would idle split their keys too.
 //
-// On B200, bf16: 8192 causal tokens of 32/8 heads of 128 in 464 us, 1.18 PFLOP/s (72 % of the measured rate); without
-// the mask 950 us, 1.16 PFLOP/s; 32 trees of 16 tokens over 400 MB of cache in 88 us.
+// On B200, bf16, device time of back-to-back replays of one input: 8192 causal tokens of 32/8 heads of 128 in 460-467 us, 1.18
+// PFLOP/s (72 % of the measured rate); without the mask 950 us, 1.16 PFLOP/s; 32 trees of 16 tokens over 400 MB of cache in
+// 90 us.  Among changing inputs, host included, the first and the last take 550 us (at the power cap) and 97-102 us.
 // The bound is the tensor pipe and, next to it, the exponentials: per 128 x 128 scores 1024 cycles of products (head
 // size 128) against 1024 of the special function unit, and a tile's softmax lies between its own two products.  So a
 // half's softmax runs beside the other half's products, and is kept short.  The running maximum moves only when a
 // row's new maximum lies more than 2^8 above it (2^4 in f16), so that O in tensor memory is rescaled rarely; probabilities
-// stay below 2^8 (2^15 in f16, scaled up by 2^11), and the sum divides the same scale out again.
+// stay below 2^8 (2^15 in f16, scaled up by 2^11), and the sum divides the same scale out again.  A probability is rounded to the
+// inputs' type for the second product, whose operands have one type; the sum takes it unrounded.  The error
+// against 64 bits is up to 1.4 times that of one rounding of the result.
 //
 // A masked score becomes -inf whatever the product holds.  A masked VALUE needs more: 0 * inf and 0 * NaN are NaN in
 // the second product, so in the tiles that are not seen whole by every row, values that are not finite are replaced by
@@ -927,7 +930,7 @@ masked_attention_kernel(const __grid_constant__ TileMaps maps, const __grid_cons
             near = __all_sync(0xFFFFFFFFu, !(big * to_vote > 0.4f));
           }
           if (near) {
-            // |s| <= 0.4 c, as almost everywhere: the short polynomial (8192 capped tokens: 755 us, 835 us without it)
+            // |s| <= 0.4 c, as almost everywhere: the short polynomial (8192 capped tokens: 730 us, 80 us more without it)
 #pragma unroll
             for (int j = 0; j < 32; j += 2) {
               const f32x2 xx = pair2(x[j], x[j + 1]);

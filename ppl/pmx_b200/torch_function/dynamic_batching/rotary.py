@@ -24,8 +24,9 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling_type: st
 
     scaling_type "": f_i = theta^(-2i/rotary_dim).  "linear": f_i / s.  "ntk": theta * s^(r/(r-2)) in the place of theta,
     which stretches the slowest pair by s and leaves the fastest alone.  "yarn": pairs that turn more than beta_fast times
-    over original_max_position stay, those that turn less than beta_slow times are divided by s, a ramp between;
-    cosine and sine take the factor 0.1 ln s + 1."""
+    over original_max_position stay, those that turn less than beta_slow times are divided by s, a ramp between
+    that is linear in the number of turns, as the method is published (a ramp that is linear in the pair's index, between the two
+    pairs that turn so often, gives other frequencies in the middle); cosine and sine take the factor 0.1 ln s + 1."""
     r, s = rotary_dim, float(scaling_factor)
     if r <= 0 or r % 2 or r > 256:
         raise ValueError(f"rotary_dim must be even, positive and at most 256, not {r}")
