@@ -368,3 +368,35 @@ def test_a_cache_without_rows_is_refused(DB):
     cache = torch.empty(0, 1, 2, 2, 64, device="cuda", dtype=torch.float16)
     with pytest.raises(ValueError, match="rows"):
         DB.tree_cache_attention(q, q, q, i64([0, 2]), i64([0]), i64([0]), i64([1, 3]), 2, 2, cache, 2, 64)
+
+
+def test_a_captured_speculative_step_follows_its_inputs(DB):
+    """Rotation by depth, tree attention and compaction in one graph: replays with other lengths, masks and accepted rows give
+    what eager calls give, with the captured bounds."""
+    rng = np.random.default_rng(11)
+    B, n, Hq, Hkv, D, rows = 3, 6, 8, 2, 128, 700
+    base = dev(cache_of(rng, 1, B * rows, 1, Hkv, D, "bf16"), "bf16")
+    x = dev(values(rng, (B * n, Hq + 2 * Hkv, D), "bf16"), "bf16")
+    ss, cs, a = i64(np.arange(B + 1) * n), i64(np.arange(B) * rows), i64([0, 2, 4, 6])
+    past, ids, mask, picks = (i64(np.zeros(m)) for m in (B, B * n, B * n, 6))
+
+    def step(cache):
+        q, k = DB.rotary_position_embedding(x[:, :Hq], x[:, Hq:Hq + Hkv], None, None, ids)
+        o = DB.tree_cache_attention(q, k, x[:, Hq + Hkv:], ss, cs, past, mask, n, 640, cache, Hq, D, num_kv_heads=Hkv, cache_layout=1)
+        DB.compact_cache(cache, cs, past, a, picks, 2, cache_layout=1)
+        return o
+    static = base.clone()
+    step(static)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for lengths in ([0, 0, 0], [600, 1, 127], [128, 0, 512]):
+        past.copy_(i64(lengths))
+        ids.copy_(i64([p + d for p in lengths for d in rng.integers(0, n, n)]))
+        mask.copy_(i64([(1 << i | int(rng.integers(0, 1 << i))) for _ in range(B) for i in range(n)]))
+        picks.copy_(i64(rng.integers(0, n, 6)))
+        static.copy_(base)
+        graph.replay()
+        eager = base.clone()
+        want = step(eager)
+        assert torch.equal(out, want) and torch.equal(static, eager)
